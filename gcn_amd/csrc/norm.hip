@@ -1,0 +1,422 @@
+// Root-mean-square norm of the rows of a layer's activations, with the residual's addition in front of it, its
+// output as float32 or as 8-bit rows with a scale each (the operand gcn_spmm_csr_quant_f32 gathers), and its
+// gradients.  The reference has no normalisation layer; the operators stand in front of its propagation step
+// (gcn/layers.py:198-202).
+//
+//   h = x + residual            inv = 1 / sqrt(mean_c h_c^2 + eps)            y_c = h_c inv w_c
+//   8 bits: scale = max(max_c |y_c| / 448, 2^-120),  q_c = e4m3(y_c / scale)       (448: the largest e4m3 value)
+//   g = w dy:  dx_c = dh_c + inv (g_c - h_c inv^2 mean_c(g h)),   dw_c = sum over rows of dy_c h_c inv
+//
+// Both directions are bound by memory: a row is read once, lives in registers between the reduction and the use of
+// its result, and is written once.  A row of f columns belongs to G lanes (G a power of two; a wave holds 64 / G
+// rows) or, past 2048 columns, to a whole workgroup; lane l holds the columns 4 (l + G j) .. + 3, so that an
+// instruction of a group reads 16 G consecutive bytes.  Sums, the maximum and the weight's gradient are float32.
+#include <algorithm>
+
+#include "common.h"
+#include "quant_rows.h"
+
+namespace gcn {
+
+constexpr int kNormMaxF = 32768;
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // 128-bit accesses at any element
+
+// columns c .. c + 3 of a row of f columns, zero past its end.  The address is moved back inside the row instead of
+// a branch around the load, so that the loads of a row stay in flight together.
+__device__ __forceinline__ void load_cols(const float* __restrict__ row, int c, int f, float (&v)[4]) {
+    if (f >= 4) {
+        const int from = c + 4 <= f ? c : f - 4;
+        const f4u t = *reinterpret_cast<const f4u*>(row + from);
+        const int gone = c - from;                 // columns of t that belong to the vector before this one
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        if (gone > 0) {
+            v[0] = gone == 1 ? t.y : gone == 2 ? t.z : gone == 3 ? t.w : 0.0f;
+            v[1] = gone == 1 ? t.z : gone == 2 ? t.w : 0.0f;
+            v[2] = gone == 1 ? t.w : 0.0f;
+            v[3] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < f ? row[c + e] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store_cols(float* __restrict__ row, int c, int f, const float (&v)[4]) {
+    if (c + 4 <= f) {
+        f4u t = {v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f4u*>(row + c) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (c + e < f) row[c + e] = v[e];
+    }
+}
+
+// sum or maximum over the G lanes of a row (G <= 64: lanes of one wave; more: the workgroup, through `lds`)
+template <int G, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* lds) {
+    constexpr int W = G < 64 ? G : 64;
+#pragma unroll
+    for (int d = W / 2; d > 0; d >>= 1) {
+        const float o = __shfl_xor(v, d);
+        v = MAX ? fmaxf(v, o) : v + o;
+    }
+    if (G > 64) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (int w = 1; w < G / 64; ++w) v = MAX ? fmaxf(v, lds[w]) : v + lds[w];
+    }
+    return v;
+}
+
+struct NormArgs {
+    int64_t n;
+    int f;
+    const float* x;
+    int64_t ldx;
+    const float* residual;   // may be null
+    int64_t ldr;
+    const float* w;          // may be null: all ones
+    float eps;
+    float* h;                // x + residual; null without a residual
+    int64_t ldh;
+    float* inv;              // [n]
+    float* y;                // float32 output, or null
+    int64_t ldy;
+    uint8_t* q;              // 8-bit output, or null
+    int64_t ldq;
+    float* scales;           // [n], with q
+};
+
+template <int G, int VPL, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
+    constexpr int kRows = BLOCK / G;                 // rows a workgroup holds at a time
+    __shared__ float lds[4][16];                     // two reductions a row, two rows before a slot is used again
+    const int sub = threadIdx.x % G;
+    const int f = a.f;
+    float w[VPL][4];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int c = 4 * (sub + G * j);
+        if (a.w && c < f) {
+            load_cols(a.w, c, f, w[j]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[j][e] = 1.0f;
+        }
+    }
+    const float inv_f = 1.0f / (float)f;
+    const int64_t base = (int64_t)blockIdx.x * tile * kRows;
+    for (int t = 0; t < tile; ++t) {
+        const int64_t i = base + (int64_t)t * kRows + threadIdx.x / G;
+        if (base + (int64_t)t * kRows >= a.n) break;                         // uniform in the workgroup
+        const bool live = i < a.n;
+        float v[VPL][4], sum = 0.0f;
+        const int64_t row = live ? i : a.n - 1;
+        const float* xr = a.x + row * a.ldx;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int c = 4 * (sub + G * j);
+            load_cols(xr, c < f ? c : 0, f, v[j]);
+        }
+        if (a.residual) {
+            const float* rr = a.residual + row * a.ldr;
+            float r[VPL][4];
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int c = 4 * (sub + G * j);
+                load_cols(rr, c < f ? c : 0, f, r[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[j][e] += r[j][e];
+                if (live && 4 * (sub + G * j) < f) store_cols(a.h + i * a.ldh, 4 * (sub + G * j), f, v[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (4 * (sub + G * j) < f) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = fmaf(v[j][e], v[j][e], sum);
+            }
+        sum = row_reduce<G, false>(sum, lds[2 * (t & 1)]);
+        const float ms = sum * inv_f;
+        const float inv = rsqrtf(ms + a.eps);
+        if (live && sub == 0) a.inv[i] = inv;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] * inv * w[j][e];
+        if (!a.q) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (live && 4 * (sub + G * j) < f) store_cols(a.y + i * a.ldy, 4 * (sub + G * j), f, v[j]);
+            continue;
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (4 * (sub + G * j) < f) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[j][e]));
+            }
+        most = row_reduce<G, true>(most, lds[2 * (t & 1) + 1]);
+        float scale = fmaxf(most * (1.0f / kE4m3Max), kQuantScaleMin);
+        // a row whose mean square or maximum is not finite has no scale: it stands for NaN as a whole
+        if (!(ms < INFINITY) || !(most < INFINITY)) scale = NAN;
+        const float up = 1.0f / scale;
+        if (live && sub == 0) a.scales[i] = scale;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int c = 4 * (sub + G * j);
+            // the bytes from f to the next multiple of 16 are part of the row and zero
+            if (live && c < ((f + 15) & ~15))
+                *reinterpret_cast<uint32_t*>(a.q + i * a.ldq + c) =
+                    e4m3_pack4(v[j][0] * up, v[j][1] * up, v[j][2] * up, v[j][3] * up, f - c);
+        }
+    }
+}
+
+struct NormGradArgs {
+    int64_t n;
+    int f;
+    const float* dy;
+    int64_t lddy;
+    const float* h;
+    int64_t ldh;
+    const float* w;          // may be null: all ones
+    const float* inv;        // [n]
+    const float* dh;         // gradient that reaches h from elsewhere; may be null
+    int64_t lddh;
+    float* dx;               // may be null
+    int64_t lddx;
+    float* part;             // [workgroups x f] partial sums of the weight's gradient, or null
+};
+
+template <int G, int VPL, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void rms_norm_grad_kernel(NormGradArgs a, int tile) {
+    constexpr int kRows = BLOCK / G;
+    __shared__ float lds[2][16];
+    __shared__ float cols[G < 256 ? (kRows - 1) * G * VPL * 4 + 1 : 1];      // weight gradients of the groups but the first
+    const int sub = threadIdx.x % G, group = threadIdx.x / G;
+    const int f = a.f;
+    float w[VPL][4], dw[VPL][4];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int c = 4 * (sub + G * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[j][e] = 1.0f;
+            dw[j][e] = 0.0f;
+        }
+        if (a.w && c < f) load_cols(a.w, c, f, w[j]);
+    }
+    const float inv_f = 1.0f / (float)f;
+    const int64_t base = (int64_t)blockIdx.x * tile * kRows;
+    for (int t = 0; t < tile; ++t) {
+        const int64_t i = base + (int64_t)t * kRows + group;
+        if (base + (int64_t)t * kRows >= a.n) break;                         // uniform in the workgroup
+        const bool live = i < a.n;
+        const int64_t row = live ? i : a.n - 1;
+        const float* dyr = a.dy + row * a.lddy;
+        const float* hr = a.h + row * a.ldh;
+        const float inv = a.inv[row];
+        float dy[VPL][4], h[VPL][4];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int c = 4 * (sub + G * j);
+            load_cols(dyr, c < f ? c : 0, f, dy[j]);
+            load_cols(hr, c < f ? c : 0, f, h[j]);
+        }
+        float along = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = 4 * (sub + G * j) < f;
+                if (in) along = fmaf(dy[j][e] * w[j][e], h[j][e], along);
+                if (in && live) dw[j][e] = fmaf(dy[j][e], h[j][e] * inv, dw[j][e]);
+            }
+        along = row_reduce<G, false>(along, lds[t & 1]);
+        const float back = along * inv_f * inv * inv;
+        if (a.dx) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int c = 4 * (sub + G * j);
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = inv * (dy[j][e] * w[j][e] - h[j][e] * back);
+                if (a.dh) {
+                    float u[4];
+                    load_cols(a.dh + row * a.lddh, c < f ? c : 0, f, u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] += u[e];
+                }
+                if (live && c < f) store_cols(a.dx + i * a.lddx, c, f, o);
+            }
+        }
+    }
+    if (!a.part) return;
+    // the groups of the workgroup in order, then one row of partial sums: no atomics, the same bits every time
+    if (G < 256 && kRows > 1) {
+        if (group > 0) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) cols[((group - 1) * VPL + j) * G * 4 + e * G + sub] = dw[j][e];
+        }
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 0; g < kRows - 1; ++g)
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dw[j][e] += cols[(g * VPL + j) * G * 4 + e * G + sub];
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int c = 4 * (sub + G * j);
+        if (c < f) store_cols(a.part + (int64_t)blockIdx.x * f, c, f, dw[j]);
+    }
+}
+
+// out[c] = sum over the rows of part [rows x f], 64 columns a workgroup, 16 strided sums a column added in order
+__global__ __launch_bounds__(1024) void column_sums_kernel(int64_t rows, int f, const float* __restrict__ part,
+                                                           float* __restrict__ out) {
+    __shared__ float lds[16][64];
+    const int col = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + col;
+    float s = 0.0f;
+    if (c < f)
+        for (int64_t r = slice; r < rows; r += 16) s += part[r * f + c];
+    lds[slice][col] = s;
+    __syncthreads();
+    if (slice == 0 && c < f) {
+        for (int k = 1; k < 16; ++k) s += lds[k][col];
+        out[c] = s;
+    }
+}
+
+int launch_column_sums(int64_t rows, int64_t f, const float* part, float* out, hipStream_t st) {
+    column_sums_kernel<<<(unsigned)ceil_div(f, (int64_t)64), 1024, 0, st>>>(rows, (int)f, part, out);
+    GCN_LAUNCH_CHECK();
+    return GCN_OK;
+}
+
+// rows a workgroup holds at a time for rows of f columns (the G, VPL and BLOCK of the launchers below)
+static inline int norm_rows(int64_t f) {
+    const int64_t vecs = ceil_div(f, (int64_t)4);
+    int g = 4;
+    while (g < 64 && g < vecs) g <<= 1;
+    return f <= 2048 ? 256 / g : 1;
+}
+
+#define GCN_NORM_BY_WIDTH(LAUNCH)              \
+    if (f <= 16) { LAUNCH(4, 1, 256); }        \
+    else if (f <= 32) { LAUNCH(8, 1, 256); }   \
+    else if (f <= 64) { LAUNCH(16, 1, 256); }  \
+    else if (f <= 128) { LAUNCH(32, 1, 256); } \
+    else if (f <= 256) { LAUNCH(64, 1, 256); } \
+    else if (f <= 512) { LAUNCH(64, 2, 256); } \
+    else if (f <= 1024) { LAUNCH(64, 4, 256); } \
+    else if (f <= 2048) { LAUNCH(64, 8, 256); } \
+    else if (f <= 4096) { LAUNCH(256, 4, 256); } \
+    else if (f <= 8192) { LAUNCH(256, 8, 256); } \
+    else if (f <= 16384) { LAUNCH(1024, 4, 1024); } \
+    else { LAUNCH(1024, 8, 1024); }
+
+// row groups a workgroup walks one after the other: one until there are workgroups for every compute unit's slots
+static inline int norm_tile(int64_t n, int64_t f) {
+    return (int)std::min<int64_t>(8, std::max<int64_t>(1, ceil_div(n, (int64_t)norm_rows(f)) / 4096));
+}
+
+// The gradient's workgroups: at most 2048, so that the partial sums of the weight's gradient stay small (2 MB at 256
+// columns) and their addition short.
+static inline int64_t norm_grad_tile(int64_t n, int64_t f) {
+    return std::max<int64_t>(1, ceil_div(ceil_div(n, (int64_t)norm_rows(f)), (int64_t)2048));
+}
+static inline int64_t norm_grad_blocks(int64_t n, int64_t f) {
+    return ceil_div(n, norm_rows(f) * norm_grad_tile(n, f));
+}
+
+static int norm_shape(int64_t n, int64_t f) {
+    if (n < 0 || f < 1 || f > kNormMaxF)
+        return fail(GCN_ERR_BAD_ARG, "bad shape: n=%lld f=%lld (a row holds 1 to %d columns)", (long long)n, (long long)f,
+                    kNormMaxF);
+    if (n > ((int64_t)1 << 32)) return fail(GCN_ERR_BAD_ARG, "more than 2^32 rows in one launch");
+    return GCN_OK;
+}
+
+}  // namespace gcn
+
+using namespace gcn;
+
+extern "C" {
+
+int gcn_quant_pitch(int64_t f, int64_t* pitch_bytes) {
+    if (!pitch_bytes || f < 1 || f > kNormMaxF) return fail(GCN_ERR_BAD_ARG, "a row holds 1 to %d columns", kNormMaxF);
+    *pitch_bytes = quant_pitch(f);
+    return GCN_OK;
+}
+
+int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const float* residual, int64_t ldr,
+                     const float* weight, float eps, float* h, int64_t ldh, float* inv, float* y, int64_t ldy,
+                     uint8_t* q, int64_t ldq, float* scales, void* stream) {
+    if (int rc = norm_shape(n, f)) return rc;
+    if (!(eps >= 0.0f)) return fail(GCN_ERR_BAD_ARG, "eps must not be negative");
+    if (ldx < f || (residual && (ldr < f || ldh < f)) || (y && ldy < f))
+        return fail(GCN_ERR_BAD_ARG, "a leading dimension is shorter than the row");
+    if (q && (ldq < (f + 15) / 16 * 16 || ldq % 16 != 0 || ((uintptr_t)q & 15) || !scales))
+        return fail(GCN_ERR_BAD_ARG, "8-bit rows want scales, a 16-byte aligned address and a pitch that is a multiple of 16 "
+                                     "not below the width: pitch %lld", (long long)ldq);
+    if (n == 0) return GCN_OK;
+    if ((y != nullptr) == (q != nullptr)) return fail(GCN_ERR_BAD_ARG, "one of the outputs y and q is wanted");
+    if (!x || !inv || (residual && !h)) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    NormArgs a = {n, (int)f, x, ldx, residual, ldr, weight, eps, h, ldh, inv, y, ldy, q, ldq, scales};
+    const int tile = norm_tile(n, f);
+    const int64_t blocks = ceil_div(n, (int64_t)norm_rows(f) * tile);
+    if (blocks > INT32_MAX) return fail(GCN_ERR_BAD_ARG, "too many rows for one launch");
+#define GCN_LAUNCH_NORM(G, VPL, BLOCK) \
+    rms_norm_kernel<G, VPL, BLOCK><<<(unsigned)blocks, BLOCK, 0, (hipStream_t)stream>>>(a, tile)
+    GCN_NORM_BY_WIDTH(GCN_LAUNCH_NORM)
+#undef GCN_LAUNCH_NORM
+    GCN_LAUNCH_CHECK();
+    return GCN_OK;
+}
+
+int gcn_rms_norm_grad_workspace_bytes(int64_t n, int64_t f, size_t* bytes) {
+    if (!bytes) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    if (int rc = norm_shape(n, f)) return rc;
+    *bytes = n ? (size_t)norm_grad_blocks(n, f) * (size_t)f * sizeof(float) : 0;
+    return GCN_OK;
+}
+
+int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, const float* h, int64_t ldh,
+                          const float* weight, const float* inv, const float* dh, int64_t lddh, float* dx, int64_t lddx,
+                          float* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = norm_shape(n, f)) return rc;
+    if (lddy < f || ldh < f || (dh && lddh < f) || (dx && lddx < f))
+        return fail(GCN_ERR_BAD_ARG, "a leading dimension is shorter than the row");
+    hipStream_t st = (hipStream_t)stream;
+    if (n == 0) return dweight ? launch_column_sums(0, f, nullptr, dweight, st) : GCN_OK;
+    if (!dy || !h || !inv) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    if (!dx && !dweight) return GCN_OK;
+    const int64_t blocks = norm_grad_blocks(n, f);
+    if (dweight) {
+        const size_t need = (size_t)blocks * (size_t)f * sizeof(float);
+        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+            return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
+    }
+    NormGradArgs a = {n, (int)f, dy, lddy, h, ldh, weight, inv, dh, lddh, dx, lddx, dweight ? (float*)workspace : nullptr};
+    const int tile = (int)norm_grad_tile(n, f);
+#define GCN_LAUNCH_NORM(G, VPL, BLOCK) \
+    rms_norm_grad_kernel<G, VPL, BLOCK><<<(unsigned)blocks, BLOCK, 0, st>>>(a, tile)
+    GCN_NORM_BY_WIDTH(GCN_LAUNCH_NORM)
+#undef GCN_LAUNCH_NORM
+    GCN_LAUNCH_CHECK();
+    return dweight ? launch_column_sums(blocks, f, (const float*)workspace, dweight, st) : GCN_OK;
+}
+
+}  // extern "C"

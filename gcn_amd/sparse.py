@@ -3,6 +3,7 @@
 torch is used for device memory and streams only; every computation is a call
 into ``libgcn_hip.so`` through ``gcn_amd._lib``.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -921,3 +922,131 @@ def gather_rows(src, rows, out):
     _lib.call('gcn_gather_rows_f32', rows.numel(), src.shape[1], src.shape[0], _p(src), _ld(src), _p(rows), _p(out),
               _ld(out), _stream())
     return out
+
+
+# --------------------------------------------------------------------------- #
+# row norm and 8-bit rows
+# --------------------------------------------------------------------------- #
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(first, *others):
+    """Context in which the device of ``first`` is the current one, so that a call enqueues on that device's current
+    stream; the other tensors must live there too."""
+    _require_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError('the tensors of one call must live on one GPU: %s and %s' % (first.device, t.device))
+    return _NO_GUARD if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+
+
+def _vector(x, n, what):
+    """A contiguous float32 vector of n elements (or None)."""
+    if x is None:
+        return None
+    if x.dim() != 1 or x.numel() != n:
+        raise ValueError('%s must be a vector of %d elements' % (what, n))
+    return x.float().contiguous()
+
+
+class QuantRows(object):
+    """A dense [n_rows x f] matrix in 8 bits: element (r, c) is ``scales[r] * e4m3(data[r, c])``.  ``data``: uint8
+    [n_rows x pitch], 16-byte aligned, the pitch a multiple of 16, the bytes from f to the next multiple of 16 zero;
+    ``scales``: float32 [n_rows].  What ``spmm_quant`` gathers instead of float32 rows: a quarter of the bytes."""
+
+    def __init__(self, n_rows, f, data, scales):
+        self.n_rows, self.f, self.data, self.scales = int(n_rows), int(f), data, scales
+        _require_cuda(data, scales)
+        if data.dtype != torch.uint8 or data.dim() != 2 or data.shape[0] != self.n_rows or data.stride(1) != 1 \
+                or data.shape[1] < (self.f + 15) // 16 * 16 or self.f < 1:
+            raise ValueError('the bytes must be a uint8 [%d x >= %d] tensor' % (self.n_rows, (self.f + 15) // 16 * 16))
+        if (self.n_rows > 1 and (data.stride(0) % 16 or data.stride(0) < data.shape[1])) or data.data_ptr() % 16:
+            raise ValueError('8-bit rows want a 16-byte aligned address and a pitch that is a multiple of 16')
+        if scales.dtype != torch.float32 or scales.shape != (self.n_rows,) or not scales.is_contiguous() \
+                or scales.device != data.device:
+            raise ValueError('the scales must be a contiguous float32 vector with one entry per row, beside the bytes')
+
+    @property
+    def ld(self):
+        return self.data.stride(0) if self.n_rows > 1 else (self.f + 15) // 16 * 16
+
+    @staticmethod
+    def pitch(f):
+        out = ctypes.c_int64()
+        _lib.call('gcn_quant_pitch', int(f), ctypes.byref(out))
+        return int(out.value)
+
+    @classmethod
+    def empty(cls, n_rows, f, device):
+        # torch's allocator returns 512-byte aligned blocks
+        return cls(n_rows, f, torch.empty((n_rows, cls.pitch(f)), dtype=torch.uint8, device=device),
+                   torch.empty(n_rows, dtype=torch.float32, device=device))
+
+    def rows(self, begin, end):
+        """Rows begin .. end - 1 as QuantRows over the same memory."""
+        return QuantRows(end - begin, self.f, self.data[begin:end], self.scales[begin:end])
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=False, out=None, sum_out=None):
+    """``(y, h, inv)`` with ``h = x + residual`` (``x`` itself without a residual), ``inv = 1 / sqrt(mean(h^2) + eps)``
+    of every row and ``y = h * inv * weight``: float32, or QuantRows with ``quant``.  One pass over the rows.
+    ``out``: where ``y`` goes (a float32 view, or QuantRows); ``sum_out``: where ``h`` goes, which may be ``x`` or
+    ``residual`` itself.  A row holds at most 32768 columns.  ``h`` and ``inv`` are what ``rms_norm_grad`` wants."""
+    with _on_device(x, weight, residual, sum_out):
+        x = _rowmajor(x)
+        n, f = x.shape
+        weight = _vector(weight, f, 'the weight')
+        h = x
+        if residual is not None:
+            residual = _rowmajor(residual)
+            if residual.shape != x.shape:
+                raise ValueError('the residual has another shape than x')
+            if sum_out is None:
+                h = torch.empty((n, f), dtype=torch.float32, device=x.device)
+            else:
+                _check_out(sum_out, n, f)
+                h = sum_out
+        elif sum_out is not None:
+            raise ValueError('sum_out without a residual: h is x itself')
+        inv = torch.empty(n, dtype=torch.float32, device=x.device)
+        if quant:
+            y = QuantRows.empty(n, f, x.device) if out is None else out
+            if not isinstance(y, QuantRows) or y.n_rows != n or y.f != f or y.data.device != x.device:
+                raise ValueError('out must be QuantRows of the shape of x')
+            args = (None, f, _p(y.data), y.ld, _p(y.scales))
+        else:
+            if out is None:
+                y = torch.empty((n, f), dtype=torch.float32, device=x.device)
+            else:
+                _check_out(out, n, f)
+                y = out
+                if y.device != x.device:
+                    raise ValueError('out lives on another GPU')
+            args = (_p(y), _ld(y), None, 0, None)
+        _lib.call('gcn_rms_norm_f32', n, f, _p(x), _ld(x), _p(residual), 0 if residual is None else _ld(residual),
+                  _p(weight), float(eps), _p(h) if residual is not None else None, _ld(h), _p(inv), *args, _stream())
+    return y, h, inv
+
+
+def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
+    """``(dx, dweight)`` of ``rms_norm``: ``grad`` is the gradient of y (of the values its 8-bit rows stand for),
+    ``h`` and ``inv`` are what the forward call returned, ``grad_h`` (may be None) the gradient that reaches h from
+    elsewhere.  ``dx`` is the gradient of x and of the residual alike.  ``dweight`` is summed over the rows in a fixed
+    order (None without ``want_weight``)."""
+    with _on_device(grad, h, weight, inv, grad_h):
+        grad, h = _rowmajor(grad), _rowmajor(h)
+        n, f = h.shape
+        if grad.shape != h.shape or (grad_h is not None and grad_h.shape != h.shape):
+            raise ValueError('shape mismatch in rms_norm_grad')
+        weight, inv = _vector(weight, f, 'the weight'), _vector(inv, n, 'inv')
+        if grad_h is not None:
+            grad_h = _rowmajor(grad_h)
+        dx = torch.empty((n, f), dtype=torch.float32, device=h.device)
+        dweight, ws, need = None, None, ctypes.c_size_t()
+        if want_weight:
+            dweight = torch.empty(f, dtype=torch.float32, device=h.device)
+            _lib.call('gcn_rms_norm_grad_workspace_bytes', n, f, ctypes.byref(need))
+            ws = _workspace(need.value, h.device)
+        _lib.call('gcn_rms_norm_grad_f32', n, f, _p(grad), _ld(grad), _p(h), _ld(h), _p(weight), _p(inv), _p(grad_h),
+                  0 if grad_h is None else _ld(grad_h), _p(dx), f, _p(dweight), _p(ws), need.value, _stream())
+    return dx, dweight

@@ -513,6 +513,42 @@ int gcn_loss_summary_f32(int64_t n, const float* row_stats, int64_t n_weights, c
 int gcn_adam_f32(int64_t n, float* param, const float* grad, float* m, float* v, float lr_t, const float* lr_t_device,
                  float beta1, float beta2, float epsilon, float weight_decay, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Row norm, 8-bit rows, distillation: pieces of deeper layers.  The           *
+ * reference has no counterpart of them; they stand next to its layer          *
+ * (gcn/layers.py:183-214) and its loss (gcn/metrics.py:85-101).                *
+ * ------------------------------------------------------------------------- */
+
+/* 8-bit rows with a scale each: element (r, c) is scales[r] * e4m3(q[r * ldq + c]).  The pitch ldq is a multiple of 16
+ * bytes, the address 16-byte aligned, and the bytes from f to the next multiple of 16 belong to the row and are zero.
+ * gcn_quant_pitch: the pitch to allocate for f <= 32768 columns -- a power of two up to 128 bytes, then a multiple
+ * of 64, so that a gathered row straddles no line it need not touch. */
+int gcn_quant_pitch(int64_t f, int64_t* pitch_bytes);
+
+/* Root-mean-square norm of every row, with the residual's addition in front of it:
+ *   h = x + residual (x itself if residual is NULL),  inv = 1 / sqrt(mean_c h_c^2 + eps),  y_c = h_c * inv * weight_c
+ * (weight NULL: all ones), f <= 32768 columns.  Written: h (only with a residual; may be x or residual itself), inv
+ * [n] (what gcn_rms_norm_grad_f32 wants), and one of
+ *   y  [n x f] float32 (may be x or residual itself where that is not also h), or
+ *   q, scales: y as 8-bit rows, scales[r] = max(max_c |y_c| / 448, 2^-120), q_c = e4m3(y_c / scales[r]) rounded to
+ *   nearest even, the bytes up to the next multiple of 16 zero.  A row whose mean square or maximum is not finite gets
+ *   the scale NaN and stands for NaN as a whole.
+ * Sums are float32: a row whose sum of squares exceeds the float32 range has inv = 0. */
+int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const float* residual, int64_t ldr,
+                     const float* weight, float eps, float* h, int64_t ldh, float* inv, float* y, int64_t ldy,
+                     uint8_t* q, int64_t ldq, float* scales, void* stream);
+
+/* Gradients of it (of the values y stands for when it was written in 8 bits): with g = weight * dy
+ *   dx_c = dh_c + inv * (g_c - h_c * inv^2 * mean_c(g h))     -- the gradient of x and of the residual alike
+ *   dweight_c = sum over rows of dy_c * h_c * inv
+ * dh (may be NULL): the gradient that reaches h itself, for a layer that hands h on.  dx (may be dy or dh itself) or
+ * dweight may be NULL.  The rows of dweight are summed in a fixed order; workspace (16-byte aligned) as the query
+ * says, not needed without dweight. */
+int gcn_rms_norm_grad_workspace_bytes(int64_t n, int64_t f, size_t* bytes);
+int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, const float* h, int64_t ldh,
+                          const float* weight, const float* inv, const float* dh, int64_t lddh, float* dx, int64_t lddx,
+                          float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

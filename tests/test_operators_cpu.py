@@ -1,0 +1,66 @@
+"""CPU: the argument checks of the row norm through the C ABI -- they return before any HIP call -- and what the
+Python operators refuse on a host without a GPU."""
+import ctypes
+
+import pytest
+
+BAD, WORKSPACE = 1, 4
+P = 4096                       # a non-null address that no call dereferences
+
+
+def _lib():
+    from gcn_amd import _lib as lib
+    return lib.load()
+
+
+def test_quant_pitch():
+    lib, out = _lib(), ctypes.c_int64()
+    for f, want in ((1, 16), (16, 16), (17, 32), (33, 64), (65, 128), (128, 128), (129, 192), (256, 256), (500, 512),
+                    (32768, 32768)):
+        assert lib.gcn_quant_pitch(f, ctypes.byref(out)) == 0 and out.value == want
+    for f in (0, -1, 32769):
+        assert lib.gcn_quant_pitch(f, ctypes.byref(out)) == BAD
+    assert lib.gcn_quant_pitch(4, None) == BAD
+
+
+def _norm(n=4, f=6, x=P, ldx=6, r=None, ldr=0, eps=1e-6, h=None, ldh=6, inv=P, y=P, ldy=6, q=None, ldq=0, scales=None):
+    return _lib().gcn_rms_norm_f32(n, f, x, ldx, r, ldr, None, eps, h, ldh, inv, y, ldy, q, ldq, scales, None)
+
+
+def test_norm_refuses():
+    assert _norm(n=0) == 0
+    for bad in (dict(n=-1), dict(f=0), dict(f=32769, ldx=32769, ldy=32769), dict(n=(1 << 32) + 1), dict(ldx=5),
+                dict(ldy=5), dict(r=P, ldr=5, h=P), dict(r=P, ldr=6, h=P, ldh=5), dict(r=P, ldr=6, h=None),
+                dict(x=None), dict(inv=None), dict(y=None), dict(q=P, ldq=16, scales=P), dict(eps=-1.0),
+                dict(eps=float('nan')), dict(y=None, q=P, ldq=16, scales=None), dict(y=None, q=P, ldq=8, scales=P),
+                dict(y=None, q=P, ldq=24, scales=P), dict(y=None, q=P + 8, ldq=16, scales=P)):
+        assert _norm(**bad) == BAD, bad
+
+
+def _norm_grad(n=4, f=6, dy=P, lddy=6, h=P, ldh=6, inv=P, dh=None, lddh=0, dx=P, lddx=6, dw=None, ws=None, nbytes=0):
+    return _lib().gcn_rms_norm_grad_f32(n, f, dy, lddy, h, ldh, None, inv, dh, lddh, dx, lddx, dw, ws, nbytes, None)
+
+
+def test_norm_gradient_refuses():
+    assert _norm_grad(n=0) == 0 and _norm_grad(dx=None) == 0
+    for bad in (dict(n=-1), dict(f=0), dict(lddy=5), dict(ldh=5), dict(dh=P, lddh=5), dict(lddx=5), dict(dy=None),
+                dict(h=None), dict(inv=None)):
+        assert _norm_grad(**bad) == BAD, bad
+    need = ctypes.c_size_t()
+    assert _lib().gcn_rms_norm_grad_workspace_bytes(4, 6, ctypes.byref(need)) == 0 and need.value >= 24
+    for bad in (dict(ws=None, nbytes=need.value), dict(ws=P, nbytes=need.value - 1), dict(ws=P + 4, nbytes=need.value)):
+        assert _norm_grad(dw=P, **bad) == WORKSPACE, bad
+    assert _lib().gcn_rms_norm_grad_workspace_bytes(4, 0, ctypes.byref(need)) == BAD
+    assert _lib().gcn_rms_norm_grad_workspace_bytes(4, 6, None) == BAD
+
+
+def test_host_tensors_are_refused():
+    import torch
+    from gcn_amd import sparse
+    if torch.cuda.is_available():
+        pytest.skip('host-only check')
+    x = torch.ones(2, 4)
+    for call in (lambda: sparse.rms_norm(x), lambda: sparse.rms_norm_grad(x, x, None, torch.ones(2)),
+                 lambda: sparse.QuantRows(2, 4, torch.zeros((2, 16), dtype=torch.uint8), torch.ones(2))):
+        with pytest.raises(ValueError):
+            call()
