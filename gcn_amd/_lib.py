@@ -23,6 +23,9 @@ GCN_RELU = 1
 GCN_SPLIT_WIDE = 4
 GCN_NORM_SYM = 0
 GCN_NORM_RW = 1
+GCN_F32 = 0
+GCN_F16 = 1
+GCN_BF16 = 2
 
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
@@ -113,6 +116,8 @@ SIGNATURES = {
     'gcn_rms_norm_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp],
     'gcn_rms_norm_grad_workspace_bytes': [_i64, _i64, _psz],
     'gcn_rms_norm_grad_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],
+    'gcn_distill_topk_f32': [_i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _i64, _i64, _vp, _f32, _f32, _vp, _vp, _vp, _i64,
+                             _vp],
 }
 
 _lib = None

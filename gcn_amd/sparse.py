@@ -1050,3 +1050,40 @@ def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
         _lib.call('gcn_rms_norm_grad_f32', n, f, _p(grad), _ld(grad), _p(h), _ld(h), _p(weight), _p(inv), _p(grad_h),
                   0 if grad_h is None else _ld(grad_h), _p(dx), f, _p(dweight), _p(ws), need.value, _stream())
     return dx, dweight
+
+
+# --------------------------------------------------------------------------- #
+# distillation
+# --------------------------------------------------------------------------- #
+_VALUE_TYPES = {torch.float32: _lib.GCN_F32, torch.float16: _lib.GCN_F16, torch.bfloat16: _lib.GCN_BF16}
+
+
+def distill_topk(logits, values, indices, mask, mask_mean, temperature=1.0, want_grad=True, want_stats=True,
+                 upstream=None):
+    """``(stats, grad)`` of the masked distillation loss from a teacher's top logits: ``values`` (float32, float16 or
+    bfloat16 [n x k], k <= 256) are the teacher's logits of the classes ``indices`` (int32 [n x k]; an index outside
+    [0, c) is no entry).  ``stats`` [n x 2]: per row ``T^2 KL(teacher || student) * w`` and the agreement of the two
+    arg maxima times ``w``, with ``w = mask / mask_mean`` (``mask`` int32 [n], None: every row) -- the rows
+    ``loss_summary`` averages; ``grad``: the gradient of their mean w.r.t. the logits, times ``upstream`` (a float32
+    device scalar) if given."""
+    with _on_device(logits, values, indices, mask, upstream):
+        logits = _rowmajor(logits)
+        n, c = logits.shape
+        if values.dtype not in _VALUE_TYPES:
+            raise ValueError("the teacher's logits must be float32, float16 or bfloat16")
+        if indices.dtype != torch.int32 or (mask is not None and mask.dtype != torch.int32):
+            raise ValueError('indices and mask must be int32')
+        if values.dim() != 2 or values.shape[0] != n or indices.shape != values.shape \
+                or (mask is not None and mask.numel() != n):
+            raise ValueError('values, indices or mask do not match the logits')
+        if upstream is not None and (upstream.dtype != torch.float32 or upstream.numel() != 1):
+            raise ValueError('upstream must be a float32 scalar')
+        values, indices = values.contiguous(), indices.contiguous()
+        mask = None if mask is None else mask.contiguous()
+        k = values.shape[1]
+        stats = torch.empty((n, 2), dtype=torch.float32, device=logits.device) if want_stats else None
+        grad = torch.empty((n, c), dtype=torch.float32, device=logits.device) if want_grad else None
+        _lib.call('gcn_distill_topk_f32', n, c, _p(logits), _ld(logits), _p(values), _VALUE_TYPES[values.dtype], k,
+                  _p(indices), k, k, _p(mask), float(mask_mean), float(temperature), _p(upstream), _p(stats), _p(grad), c,
+                  _stream())
+    return stats, grad

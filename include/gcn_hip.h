@@ -45,6 +45,10 @@ typedef enum {
 #define GCN_RELU 1            /* act = relu fused into the epilogue                  (gcn/layers.py:214, models.py:17) */
 #define GCN_SPLIT_WIDE 4      /* spmm: cut long rows every 1024 entries whatever the width, so that a product
                                  computed over ranges of feature columns equals the full-width one bit for bit */
+/* element types of stored values */
+#define GCN_F32 0
+#define GCN_F16 1
+#define GCN_BF16 2
 /* type of gcn_normalize_adj */
 #define GCN_NORM_SYM 0        /* D^-1/2 A D^-1/2                                     (gcn/utils.py:299-308) */
 #define GCN_NORM_RW 1         /* D^-1 A                                              (gcn/utils.py:309-315) */
@@ -548,6 +552,22 @@ int gcn_rms_norm_grad_workspace_bytes(int64_t n, int64_t f, size_t* bytes);
 int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, const float* h, int64_t ldh,
                           const float* weight, const float* inv, const float* dh, int64_t lddh, float* dx, int64_t lddx,
                           float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits under the reference's mask (gcn/metrics.py:85-92), with the gradient
+ * optimizer.minimize (gcn/models.py:86) would derive.  Row i lists k <= 256 teacher logits (value_type GCN_F32, GCN_F16 or
+ * GCN_BF16) with their classes; an index outside [0, c) is no entry, a class listed more than once counts every time.
+ * With p = softmax(listed / T), q = softmax(logits / T) over all c classes and w_i = mask_i / mask_mean (mask NULL: ones):
+ *   row_stats [n x 2] (may be NULL, 8-byte aligned): (T^2 sum_j p_j (log p_j - log q_idx_j) * w_i,
+ *       w_i where the row's first maximum is the class of the largest listed logit -- of equal ones the first listed --,
+ *       else 0): the rows gcn_loss_summary_f32 averages
+ *   dlogits [n x c] (may be NULL; must not overlap the logits): (q_c - P_c) * T * w_i / n [* *upstream], P_c the sum of
+ *       the p_j listed at class c.  upstream (device scalar, may be NULL) is read when the kernel runs.
+ * Rows with mask 0 are not read and rows without an entry (or with listed logits of -inf only) have no loss: both get
+ * zeros.  A NaN or +inf in a row of the mask makes that row NaN; a logit of -inf at a listed class makes its loss +inf. */
+int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx, const void* values, int value_type,
+                         int64_t ldv, const int32_t* indices, int64_t ldi, int64_t k, const int32_t* mask, float mask_mean,
+                         float temperature, const float* upstream, float* row_stats, float* dlogits, int64_t ldd,
+                         void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,4 +1,4 @@
-"""CPU: the argument checks of the row norm through the C ABI -- they return before any HIP call -- and what the
+"""CPU: the argument checks of the row norm and the distillation loss through the C ABI -- they return before any HIP call -- and what the
 Python operators refuse on a host without a GPU."""
 import ctypes
 
@@ -54,6 +54,20 @@ def test_norm_gradient_refuses():
     assert _lib().gcn_rms_norm_grad_workspace_bytes(4, 6, None) == BAD
 
 
+def _distill(n=4, c=6, x=P, ldx=6, v=P, vt=0, ldv=3, i=P, ldi=3, k=3, mask=P, mean=0.5, temp=1.0, up=None, stats=P, d=P,
+             ldd=6):
+    return _lib().gcn_distill_topk_f32(n, c, x, ldx, v, vt, ldv, i, ldi, k, mask, mean, temp, up, stats, d, ldd, None)
+
+
+def test_distillation_refuses():
+    assert _distill(n=0) == 0 and _distill(stats=None, d=None) == 0
+    for bad in (dict(n=-1), dict(c=0), dict(c=2 ** 31, ldx=2 ** 31, ldd=2 ** 31), dict(ldx=5), dict(ldd=5), dict(k=0),
+                dict(k=257, ldv=257, ldi=257), dict(ldv=2), dict(ldi=2), dict(vt=3), dict(mean=0.0), dict(mean=float('nan')),
+                dict(temp=0.0), dict(temp=-1.0), dict(temp=float('inf')), dict(temp=float('nan')), dict(x=None), dict(v=None),
+                dict(i=None), dict(stats=P + 4)):
+        assert _distill(**bad) == BAD, bad
+
+
 def test_host_tensors_are_refused():
     import torch
     from gcn_amd import sparse
@@ -61,6 +75,6 @@ def test_host_tensors_are_refused():
         pytest.skip('host-only check')
     x = torch.ones(2, 4)
     for call in (lambda: sparse.rms_norm(x), lambda: sparse.rms_norm_grad(x, x, None, torch.ones(2)),
-                 lambda: sparse.QuantRows(2, 4, torch.zeros((2, 16), dtype=torch.uint8), torch.ones(2))):
+                 lambda: sparse.distill_topk(x, x, x.int(), None, 1.0), lambda: sparse.QuantRows(2, 4, torch.zeros((2, 16), dtype=torch.uint8), torch.ones(2))):
         with pytest.raises(ValueError):
             call()
