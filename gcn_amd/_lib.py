@@ -116,6 +116,7 @@ SIGNATURES = {
     'gcn_rms_norm_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp],
     'gcn_rms_norm_grad_workspace_bytes': [_i64, _i64, _psz],
     'gcn_rms_norm_grad_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],
+    'gcn_spmm_csr_quant_f32': [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _sz, _vp],
     'gcn_distill_topk_f32': [_i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _i64, _i64, _vp, _f32, _f32, _vp, _vp, _vp, _i64,
                              _vp],
 }

@@ -22,33 +22,7 @@
 #include <vector>
 
 #include "common.h"
-
-struct gcn_spmm_plan {
-    int64_t n_rows, n_cols, nnz;
-    int64_t n_strips;
-    int strip_nnz;       // entries per strip
-    int chunk_len;       // entries per chunk of a long row; 0: the split threshold itself
-    int split[2];        // rows longer than this are summed chunk-wise (narrow / wide dense operands)
-    int device;
-    int32_t* strip_row;  // [n_strips + 1] first row starting in each strip
-    // rows longer than the split threshold, cut in chunks of that many entries; table 0 serves narrow
-    // dense operands (threshold kSplitNarrow), table 1 wide ones (kSplitWide)
-    struct LongTable {
-        int64_t n_long, n_chunks;
-        int32_t* long_row;    // [n_long] ascending
-        int64_t* long_chunk;  // [n_long + 1] first chunk of each long row
-        int32_t* chunk_long;  // [n_chunks] long-row slot of each chunk
-    } table[2];
-    // columns >= hot_cols are loaded with the non-temporal hint by the wave-per-row instances (0: off).
-    // After a degree-descending relabel the first columns are the hub rows of B: the rows worth caching.
-    int64_t hot_cols;
-    // narrow products stage the first lds_hub_rows rows of B in LDS, once per workgroup, and entries whose
-    // column is below that number read them from there (0: off).  For a degree-ordered matrix those are the
-    // hub rows: the "LDS-staged row-block" form of the product.
-    int64_t lds_hub_rows;
-    int timing;           // record events around the kernels of every product
-    hipEvent_t ev[3];     // start, after the row kernel, after the long-row reduction
-};
+#include "spmm_plan.h"
 
 // Scratch of gcn_spmm_csr_f32_noalloc: the partial rows of long-row chunks, which the other entry
 // points take from a caller workspace.  One copy per GPU the library runs on, held until the process
@@ -731,18 +705,6 @@ __device__ __forceinline__ void chunks_block(int64_t block, int64_t n_chunks, co
         store_row<VEC, VPL>(part + chunk * ldp, nullptr, col, on, acc, false, none, 0);
     }
 }
-
-struct PlanView {
-    int64_t n_strips, n_chunks, chunk_blocks, nnz;
-    int split;
-    int chunk_len;
-    uint32_t hot_cols;
-    uint32_t lds_hub_rows;
-    const int32_t* strip_row;
-    const int32_t* chunk_long;
-    const int32_t* long_row;
-    const int64_t* long_chunk;
-};
 
 // The whole product in one launch: the blocks that sum chunks of long rows come first (they are
 // the longest work items), the strip blocks after them.
@@ -1508,6 +1470,15 @@ static int launch_by_width(const SpmmCall& a) {
     return launch_variant<64, VEC, 2, DROPOUT>(a);  // wider rows: passes of 128 vectors
 }
 
+int launch_long_reduce(const gcn_spmm_plan::LongTable& lt, int64_t f, const float* part, int64_t ldp, float* c, int64_t ldc,
+                       int relu, int vec_c, hipStream_t st) {
+    const OutDrop none = {0, 1.0f, 0, 0, nullptr, 0, 0};
+    spmm_long_reduce_kernel<<<(unsigned)ceil_div(lt.n_long, kBlock / 64), kBlock, 0, st>>>(
+        lt.n_long, lt.long_row, lt.long_chunk, f, part, ldp, c, ldc, relu, vec_c, nullptr, 0, none);
+    GCN_LAUNCH_CHECK();
+    return GCN_OK;
+}
+
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 static inline int64_t partial_ld(int64_t f) { return (f + 3) / 4 * 4; }
@@ -2048,12 +2019,8 @@ int gcn_spmm_csr_packed_f32(const gcn_spmm_plan* plan, const int64_t* indptr, co
                                                                       (uint32_t)ldpk, c, ldc, c_vec, part, ldp, relu);
     GCN_LAUNCH_CHECK();
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[1], st));
-    if (lt.n_chunks > 0) {
-        const OutDrop none = {0, 1.0f, 0, 0, nullptr, 0, 0};
-        spmm_long_reduce_kernel<<<(unsigned)ceil_div(lt.n_long, kWaves), kBlock, 0, st>>>(
-            lt.n_long, lt.long_row, lt.long_chunk, f, part, ldp, c, ldc, relu, c_vec, nullptr, 0, none);
-        GCN_LAUNCH_CHECK();
-    }
+    if (lt.n_chunks > 0)
+        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu, c_vec, st)) return rc;
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[2], st));
     return GCN_OK;
 }

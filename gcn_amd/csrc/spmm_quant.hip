@@ -1,0 +1,239 @@
+// CSR x 8-bit rows (quant_rows.h): C = act(A . B) with B[r, c] = scales[r] e4m3(q[r, c]), the propagation step
+// dot(support, ., sparse=True) of a layer (gcn/layers.py:202) on an operand a quarter as wide.
+//
+//   C[i, :] = act(sum_e (a_e s[col_e]) q[col_e, :])        float32 sums, one fused multiply-add an element
+//
+// The product is bound by the rows it gathers: at 256 columns 256 bytes an entry (two 128-byte lines) and the entry's
+// scale, instead of the 1024 bytes of float32 rows.  A wave takes the strips of rows the plan cut, one row after the
+// other.  L lanes hold 16 columns each (one 16-byte load a row), so 64 / L entries of the row are gathered by one
+// instruction; each lane group adds its entries, and at the end of a row the groups are added by exchanging halves: after
+// the exchange over lane distance 32 a lane is left with 8 of its 16 columns, then 4, 2, 1.  64 (column, value)
+// pairs of a row are read by one load each, a lane an entry, with the gather of their scales; the lanes' entries
+// then reach the groups by shuffles.  Long rows are cut at the chunks of the wide dense product and joined in chunk order.
+#include <algorithm>
+
+#include "common.h"
+#include "quant_rows.h"
+#include "spmm_plan.h"
+
+namespace gcn {
+
+constexpr int kBlock = 256;
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// acc += w * (the 16 values of a 16-byte piece)
+__device__ __forceinline__ void add_piece(const uint4& raw, float w, float (&acc)[16]) {
+    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)words[i], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)words[i], true);
+        acc[4 * i] = fmaf(w, lo.x, acc[4 * i]);
+        acc[4 * i + 1] = fmaf(w, lo.y, acc[4 * i + 1]);
+        acc[4 * i + 2] = fmaf(w, hi.x, acc[4 * i + 2]);
+        acc[4 * i + 3] = fmaf(w, hi.y, acc[4 * i + 3]);
+    }
+}
+
+// Adds the lane groups of L lanes: the lane is left with kLeft(L) sums of its 16 columns, from column `offset` on.
+constexpr int left_of(int L) { return L >= 64 ? 16 : L == 32 ? 8 : L == 16 ? 4 : L == 8 ? 2 : 1; }
+template <int L>
+__device__ __forceinline__ int add_groups(float (&acc)[16], int lane) {
+    int offset = 0;
+    if (L <= 32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i + 8]), false, false);
+            acc[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        }
+        offset += (lane & 32) ? 8 : 0;
+    }
+    if (L <= 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i + 4]), false, false);
+            acc[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        }
+        offset += (lane & 16) ? 4 : 0;
+    }
+    if (L <= 8) {
+        const bool up = lane & 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float give = up ? acc[i] : acc[i + 2], keep = up ? acc[i + 2] : acc[i];
+            acc[i] = keep + __shfl_xor(give, 8);
+        }
+        offset += up ? 2 : 0;
+    }
+    if (L <= 4) {
+        const bool up = lane & 4;
+        const float give = up ? acc[0] : acc[1], keep = up ? acc[1] : acc[0];
+        acc[0] = keep + __shfl_xor(give, 4);
+        offset += up ? 1 : 0;
+    }
+    if (L <= 2) acc[0] += __shfl_xor(acc[0], 2);
+    if (L <= 1) acc[0] += __shfl_xor(acc[0], 1);
+    return offset;
+}
+
+// sums of the entries k0 .. k1 - 1, this lane's 16 columns, before the groups are added
+template <int L>
+__device__ __forceinline__ void accumulate_quant(int64_t k0, int64_t k1, const int32_t* __restrict__ indices,
+                                                 const float* __restrict__ vals, const uint8_t* __restrict__ q, uint32_t ldq,
+                                                 const float* __restrict__ scales, int lane, int64_t piece,
+                                                 float (&acc)[16]) {
+    constexpr int P = 64 / L;              // entries a step gathers
+    constexpr int U = 4;                   // steps in flight
+    const int group = lane / L;
+    for (int64_t k = k0; k < k1; k += 64) {
+        // lanes past the end repeat the last entry with weight 0: its row is read anyway
+        const int64_t e = k + lane < k1 ? k + lane : k1 - 1;
+        const int32_t col = indices[e];
+        float w = vals[e] * scales[col];
+        if (k + lane >= k1) w = 0.0f;
+        const int n = (int)(k1 - k < 64 ? k1 - k : 64);
+        const int steps = (n + P - 1) / P;
+        for (int s = 0; s < steps; s += U) {
+            uint4 raw[U];
+            float ws[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int from = min((s + u) * P + group, 63);
+                const int32_t c = __shfl(col, from);
+                ws[u] = __shfl(w, from);
+                if (s + u >= steps) ws[u] = 0.0f;
+                raw[u] = *reinterpret_cast<const uint4*>(q + (uint64_t)(uint32_t)c * ldq + piece);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) add_piece(raw[u], ws[u], acc);
+        }
+    }
+}
+
+template <int L>
+__global__ __launch_bounds__(kBlock) void spmm_quant_kernel(PlanView pv, const int64_t* __restrict__ indptr,
+                                                            const int32_t* __restrict__ indices,
+                                                            const float* __restrict__ vals, int f,
+                                                            const uint8_t* __restrict__ q, uint32_t ldq,
+                                                            const float* __restrict__ scales, float* __restrict__ c,
+                                                            int64_t ldc, int c_vec, float* __restrict__ part, int64_t ldp,
+                                                            int relu) {
+    constexpr int kLeft = left_of(L);
+    const int lane = threadIdx.x & 63, sub = lane % L;
+    const int col0 = (int)blockIdx.y * 16 * L + 16 * sub;           // this lane's columns
+    const int64_t piece = col0 < f ? col0 : (int64_t)blockIdx.y * 16 * L;
+    const int64_t block = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    auto finish = [&](float (&acc)[16], float* row, bool vec, bool act) {
+        const int at = col0 + add_groups<L>(acc, lane);
+        if (L < 4 && (lane & 3 & ~(L - 1))) return;                 // L = 1, 2: the groups past the fourth hold the same sum
+#pragma unroll
+        for (int i = 0; i < kLeft; ++i)
+            if (act) acc[i] = acc[i] > 0.0f ? acc[i] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLeft; i += 4) {
+            if (kLeft >= 4 && vec && at + i + 4 <= f) {
+                *reinterpret_cast<float4*>(row + at + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4 && i + e < kLeft; ++e)
+                    if (at + i + e < f) row[at + i + e] = acc[i + e];
+            }
+        }
+    };
+    if (block < pv.chunk_blocks) {
+        const int64_t chunk = block * (kBlock / 64) + wave;
+        if (chunk >= pv.n_chunks) return;
+        const int li = pv.chunk_long[chunk];
+        const int r = pv.long_row[li];
+        const int64_t k0 = indptr[r] + (chunk - pv.long_chunk[li]) * (int64_t)pv.chunk_len;
+        const int64_t row_end = indptr[r + 1];
+        const int64_t k1 = k0 + pv.chunk_len < row_end ? k0 + pv.chunk_len : row_end;
+        float acc[16] = {};
+        accumulate_quant<L>(k0, k1, indices, vals, q, ldq, scales, lane, piece, acc);
+        finish(acc, part + chunk * ldp, true, false);               // partial rows: 16-byte aligned, pitch a multiple of 4
+        return;
+    }
+    const int64_t strip = (block - pv.chunk_blocks) * (kBlock / 64) + wave;
+    if (strip >= pv.n_strips) return;
+    const int r_hi = pv.strip_row[strip + 1];
+    for (int r = pv.strip_row[strip]; r < r_hi; ++r) {
+        const int64_t k0 = indptr[r], k1 = indptr[r + 1];
+        if (k1 - k0 > pv.split) continue;                           // summed chunk-wise
+        float acc[16] = {};
+        accumulate_quant<L>(k0, k1, indices, vals, q, ldq, scales, lane, piece, acc);
+        finish(acc, c + (int64_t)r * ldc, c_vec != 0, relu != 0);
+    }
+}
+
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace gcn
+
+using namespace gcn;
+
+extern "C" {
+
+int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, const int32_t* indices, const float* vals,
+                           int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* c, int64_t ldc, int flags,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    if (!plan) return fail(GCN_ERR_BAD_ARG, "plan is null");
+    if (f < 1 || f > 32768) return fail(GCN_ERR_BAD_ARG, "an 8-bit row holds 1 to 32768 columns: f=%lld", (long long)f);
+    if (ldc < f || ldq < (f + 15) / 16 * 16 || ldq % 16 != 0 || ldq > INT32_MAX)
+        return fail(GCN_ERR_BAD_ARG, "bad pitch: ldc=%lld, 8-bit pitch %lld", (long long)ldc, (long long)ldq);
+    if (!indptr || (plan->nnz > 0 && (!indices || !vals))) return fail(GCN_ERR_BAD_ARG, "null CSR pointer");
+    if (flags & ~GCN_RELU) return fail(GCN_ERR_BAD_ARG, "unknown flag bits 0x%x", flags);
+    if (plan->n_rows == 0) return GCN_OK;
+    if (!c || (plan->nnz > 0 && (!q || !scales))) return fail(GCN_ERR_BAD_ARG, "null dense pointer");
+    if (!aligned16(q)) return fail(GCN_ERR_BAD_ARG, "8-bit rows must be 16-byte aligned");
+    const gcn_spmm_plan::LongTable& lt = plan->table[1];            // the cut points of the wide dense product
+    constexpr int kWaves = kBlock / 64;
+    PlanView pv;
+    pv.n_strips = plan->n_strips;
+    pv.nnz = plan->nnz;
+    pv.n_chunks = lt.n_chunks;
+    pv.chunk_blocks = ceil_div(lt.n_chunks, kWaves);
+    pv.split = plan->split[1];
+    pv.chunk_len = plan->chunk_len ? plan->chunk_len : pv.split;
+    pv.hot_cols = 0;
+    pv.lds_hub_rows = 0;
+    pv.strip_row = plan->strip_row;
+    pv.chunk_long = lt.chunk_long;
+    pv.long_row = lt.long_row;
+    pv.long_chunk = lt.long_chunk;
+    float* part = nullptr;
+    const int64_t ldp = (f + 3) / 4 * 4;
+    if (lt.n_chunks > 0) {
+        const size_t need = (size_t)lt.n_chunks * (size_t)ldp * sizeof(float);
+        if (!workspace || workspace_bytes < need)
+            return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+        if (!aligned16(workspace)) return fail(GCN_ERR_BAD_ARG, "workspace must be 16-byte aligned");
+        part = (float*)workspace;
+    }
+    const int64_t grid = pv.chunk_blocks + ceil_div(plan->n_strips, kWaves);
+    if (grid >= (int64_t)1 << 24) return fail(GCN_ERR_BAD_ARG, "matrix too large for one launch");   // threads count in 32 bits
+    hipStream_t st = (hipStream_t)stream;
+    const int relu = (flags & GCN_RELU) ? 1 : 0;
+    const int c_vec = (ldc % 4 == 0 && aligned16(c)) ? 1 : 0;
+    if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[0], st));
+#define GCN_QUANT_GO(L)                                                                                                  \
+    spmm_quant_kernel<L><<<dim3((unsigned)grid, (unsigned)ceil_div(f, (int64_t)16 * L)), kBlock, 0, st>>>(               \
+        pv, indptr, indices, vals, (int)f, q, (uint32_t)ldq, scales, c, ldc, c_vec, part, ldp, relu)
+    if (f <= 16) GCN_QUANT_GO(1);
+    else if (f <= 32) GCN_QUANT_GO(2);
+    else if (f <= 64) GCN_QUANT_GO(4);
+    else if (f <= 128) GCN_QUANT_GO(8);
+    else if (f <= 256) GCN_QUANT_GO(16);
+    else if (f <= 512) GCN_QUANT_GO(32);
+    else GCN_QUANT_GO(64);                                           // wider rows: ranges of 1024 columns
+#undef GCN_QUANT_GO
+    GCN_LAUNCH_CHECK();
+    if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[1], st));
+    if (lt.n_chunks > 0)
+        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu, c_vec && f % 4 == 0, st)) return rc;
+    if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[2], st));
+    return GCN_OK;
+}
+
+}  // extern "C"

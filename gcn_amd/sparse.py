@@ -1052,6 +1052,29 @@ def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
     return dx, dweight
 
 
+def spmm_quant(a, q, relu=False, out=None):
+    """``a @ B`` (optionally with ReLU) for the matrix B that the QuantRows ``q`` stand for, gathering their 8-bit rows.
+    float32 sums in a fixed order (not the serial order of ``spmm``).  The workspace of long rows belongs to the call, so
+    products on several streams, or recorded in several graphs, do not share one."""
+    if not isinstance(q, QuantRows):
+        raise ValueError('spmm_quant takes QuantRows')
+    with _on_device(q.data, a.indptr, out):
+        if q.n_rows != a.n_cols:
+            raise ValueError('shape mismatch: %s @ 8-bit [%d x %d]' % (a.shape, q.n_rows, q.f))
+        f = q.f
+        if out is None:
+            out = torch.empty((a.n_rows, f), dtype=torch.float32, device=q.data.device)
+        else:
+            _check_out(out, a.n_rows, f)
+        need, ws = ctypes.c_size_t(), None
+        _lib.call('gcn_spmm_plan_workspace_bytes', a.plan.handle, f, ctypes.byref(need))
+        if need.value:
+            ws = _workspace(need.value, q.data.device)
+        _lib.call('gcn_spmm_csr_quant_f32', a.plan.handle, _p(a.indptr), _p(a.indices), _p(a.values), f, _p(q.data), q.ld,
+                  _p(q.scales), _p(out), _ld(out), _lib.GCN_RELU if relu else 0, _p(ws), need.value, _stream())
+    return out
+
+
 # --------------------------------------------------------------------------- #
 # distillation
 # --------------------------------------------------------------------------- #
