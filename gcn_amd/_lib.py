@@ -23,6 +23,10 @@ GCN_RELU = 1
 GCN_SPLIT_WIDE = 4
 GCN_NORM_SYM = 0
 GCN_NORM_RW = 1
+GCN_ACT_NONE = 0
+GCN_ACT_RELU = 1
+GCN_ACT_GELU = 2
+GCN_ACT_SILU = 3
 GCN_F32 = 0
 GCN_F16 = 1
 GCN_BF16 = 2
@@ -117,6 +121,11 @@ SIGNATURES = {
     'gcn_rms_norm_grad_workspace_bytes': [_i64, _i64, _psz],
     'gcn_rms_norm_grad_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],
     'gcn_spmm_csr_quant_f32': [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _sz, _vp],
+    'gcn_gemm_epilogue_workspace_bytes': [_i64, _i64, _i64, _psz],
+    'gcn_gemm_epilogue_f32': [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _int, _vp, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                              _sz, _vp],
+    'gcn_act_grad_workspace_bytes': [_i64, _i64, _psz],
+    'gcn_act_grad_f32': [_i64, _i64, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],
     'gcn_distill_topk_f32': [_i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _i64, _i64, _vp, _f32, _f32, _vp, _vp, _vp, _i64,
                              _vp],
 }

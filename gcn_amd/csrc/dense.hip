@@ -4,6 +4,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "activations.h"
 #include "common.h"
 
 namespace gcn {
@@ -180,15 +181,77 @@ __global__ void gather_rows_kernel(int64_t n_out, int64_t f, const float* __rest
 // ------------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// The store of a dense layer's tile: C = act(acc + bias) + residual, the pre-activation to pre.  Every access is a buffer
+// instruction on a range that ends with the tile's last element, and the lanes of columns past n point behind it: the
+// hardware returns 0 there and drops the stores, so the edge tiles need no branches.  (With a test per element the
+// 128 x 128 tile spilled 222 registers.)  The residual of a 32 x 32 block is requested before the block's first store.
+// Offsets stay below 2^31: leading dimensions are limited to 2^22 - 1 by the callers.
+template <int MT, int NT>
+__device__ __forceinline__ void store_layer_tile(const f32x16 (&acc)[MT][NT], const EpiArgs& ep, float* c, int64_t ldc, int64_t m0,
+                                                 int64_t n0, int m_left, int n_left, int row_in, int col_in, int lane) {
+    auto range = [&](const float* base, int64_t ld) {
+        const int bytes = base ? ((m_left - 1) * (int)ld + n_left) * 4 : 0;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base ? base + m0 * ld + n0 : nullptr), 0, bytes, 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t res_c = range(c, ldc), res_r = range(ep.residual, ep.ldr), res_p = range(ep.pre, ep.ldp);
+    const int l31 = lane & 31, row0 = row_in + 4 * (lane >> 5);
+    with_act(ep.act, [&](auto which) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int col = col_in + 32 * j + l31;
+            const uint32_t past = col < n_left ? 0u : 0x80000000u;
+            const float add = ep.bias && col < n_left ? ep.bias[n0 + col] : 0.0f;
+            const uint32_t at_c = (uint32_t)(row0 * (int)ldc + col) * 4u + past, at_r = (uint32_t)(row0 * (int)ep.ldr + col) * 4u + past,
+                           at_p = (uint32_t)(row0 * (int)ep.ldp + col) * 4u + past;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float rv[16];
+                if (ep.residual) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int row = i * 32 + (e & 3) + 8 * (e >> 2);
+                        rv[e] = __uint_as_float(
+                            __builtin_amdgcn_raw_buffer_load_b32(res_r, (int)(at_r + (uint32_t)(row * (int)ep.ldr) * 4u), 0, 0));
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = i * 32 + (e & 3) + 8 * (e >> 2);
+                    const float z = acc[i][j][e] + add;
+                    if (ep.pre)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(z), res_p,
+                                                              (int)(at_p + (uint32_t)(row * (int)ep.ldp) * 4u), 0, 0);
+                    float v = act_value<decltype(which)::value>(z);
+                    if (ep.residual) v += rv[e];
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), res_c,
+                                                          (int)(at_c + (uint32_t)(row * (int)ldc) * 4u), 0, 0);
+                }
+            }
+        }
+    });
+}
+
 // kBK = 32, or 16 for products whose whole K fits 16 (hidden -> classes)
-template <int kBM, int BN, bool TRANS_B, int kBK>
+// LAYER: the store is a dense layer's epilogue (EpiArgs) -- or, with k_cut > 0, the bare partial product of the k range
+// that grid y names, which launch_join_splits adds up: a product of few tiles and a long k is then not one workgroup's walk.
+template <int kBM, int BN, bool TRANS_B, int kBK, bool LAYER = false>
 __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t n, int64_t k,
                                                            const float* __restrict__ a, int64_t lda,
                                                            const float* __restrict__ b, int64_t ldb,
                                                            float* __restrict__ c, int64_t ldc, int relu, int a_vec,
                                                            int b_vec, int64_t tiles_m, int64_t tiles_n,
                                                            const float* __restrict__ gate, int64_t ldg,
-                                                           float divisor, OutDrop od, InMask im) {
+                                                           float divisor, OutDrop od, InMask im, EpiArgs ep,
+                                                           int64_t k_cut) {
+    if constexpr (LAYER) {
+        if (k_cut > 0) {
+            const int64_t from = (int64_t)blockIdx.y * k_cut;
+            a += from;
+            b += TRANS_B ? from : from * ldb;
+            c += (int64_t)blockIdx.y * m * n;
+            k = k - from < k_cut ? k - from : k_cut;
+        }
+    }
     constexpr int kWavesN = (BN >= 64) ? 2 : 1;
     constexpr int kWavesM = 4 / kWavesN;
     constexpr int MT = kBM / (kWavesM * 32);
@@ -413,6 +476,13 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
         __syncthreads();
     }
     // C/D layout of the 32x32 MFMA: col = lane & 31, row = (reg & 3) + 8 * (reg >> 2) + 4 * (lane >> 5)
+    if constexpr (LAYER) {
+        if (k_cut == 0) {
+            store_layer_tile<MT, NT>(acc, ep, c, ldc, m0, n0, (int)(m - m0 < kBM ? m - m0 : kBM),
+                                     (int)(n - n0 < BN ? n - n0 : BN), wm * MT * 32, wn * NT * 32, lane);
+            return;
+        }
+    }
     if (gate) {
         // C = gate > 0 ? (A.B) / divisor : 0 -- the backward of dropout(relu(.)) folded into the product
         // that computes the gradient of its output (gate = that output: positive where the unit was
@@ -554,7 +624,7 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
 //    passes as itself (tested on rows that hold NaN, both infinities and negative underflow).
 // ------------------------------------------------------------------------------------------------
 typedef float f32x4v __attribute__((ext_vector_type(4)));
-enum { kEpiPlain = 0, kEpiGate = 1, kEpiDrop = 2 };
+enum { kEpiPlain = 0, kEpiGate = 1, kEpiDrop = 2, kEpiLayer = 3 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t whole_range_buffer(const void* base) {
     // raw buffer (stride 0), no range clamp below 4 GiB, 32-bit data format
@@ -581,7 +651,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
                                                                const float* __restrict__ b, int64_t ldb,
                                                                float* __restrict__ c, int64_t ldc, int relu,
                                                                const float* __restrict__ gate, int64_t ldg,
-                                                               float divisor, InMask im, OutDrop od, int raster) {
+                                                               float divisor, InMask im, OutDrop od, int raster,
+                                                               EpiArgs ep) {
     constexpr int kBM = 128, BN = 128, kBK = 32, MT = 2, NT = 2;
     constexpr int kAPitch = kBK + 4, kBPitch = BN + 4;
     __shared__ __attribute__((aligned(16))) float as[kBM * kAPitch];
@@ -778,6 +849,10 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
             gated_store(std::false_type{});
         return;
     }
+    if (EPI == kEpiLayer) {
+        store_layer_tile<MT, NT>(acc, ep, c, ldc, m0, n0, kBM, BN, wm * MT * 32, wn * NT * 32, lane);
+        return;
+    }
     if (EPI == kEpiDrop) {
         // C = dropout(act(A.B)): decision id = index_offset + drawn row * pitch + column.  The four lanes of a
         // quad hold four consecutive columns of the same rows, i.e. (when pitch and index_offset are multiples
@@ -875,13 +950,15 @@ static bool panels_form_fits(int64_t m, int64_t n, int64_t k, const float* a, in
 }
 
 static const InMask kNoInMask = {nullptr, 0, 1.0f, 1.0f, 1};
+static const EpiArgs kNoEpi = {nullptr, nullptr, 0, nullptr, 0, GCN_ACT_NONE};
 
 template <int kBM, int BN>
 static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
                        int trans_b, float* c, int64_t ldc, int relu, hipStream_t st, const float* gate = nullptr,
                        int64_t ldg = 0, float divisor = 1.0f, const OutDrop* out_drop = nullptr,
-                       const InMask* in_mask = nullptr) {
+                       const InMask* in_mask = nullptr, const EpiArgs* layer = nullptr) {
     const InMask im = in_mask ? *in_mask : kNoInMask;
+    const EpiArgs ep = layer ? *layer : kNoEpi;
     const OutDrop no_drop = {0, 1.0f, 0, 0, nullptr, 0, 0, nullptr, 0};
     // the byte offset of a mask word inside a panel's buffer stays below 2^31 like every other offset
     const bool mask_fits = !im.bits || (!trans_b && !gate && !out_drop && 128 * im.ld_words + k / 32 < ((int64_t)1 << 29));
@@ -894,9 +971,14 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
         const int raster = n / 128 >= 16 ? 1 : 0;
 #define GCN_PANELS_GO(TB, EPI, AM)                                                                                \
     gemm_panels_kernel<TB, EPI, AM><<<grid, kBlock, 0, st>>>((int)panels, (int)(k / 32), a, lda, b, ldb, c, ldc, relu, gate, \
-                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster)
+                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster, ep)
         if (im.bits) {
             GCN_PANELS_GO(false, kEpiPlain, true);
+        } else if (layer) {
+            if (trans_b)
+                GCN_PANELS_GO(true, kEpiLayer, false);
+            else
+                GCN_PANELS_GO(false, kEpiLayer, false);
         } else if (out_drop) {
             if (trans_b)
                 GCN_PANELS_GO(true, kEpiDrop, false);
@@ -927,9 +1009,12 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
         }
         InMask rest_mask = im;
         if (im.bits) rest_mask.bits += done * im.ld_words;
+        EpiArgs rest_layer = ep;
+        if (ep.residual) rest_layer.residual += done * ep.ldr;
+        if (ep.pre) rest_layer.pre += done * ep.ldp;
         return launch_gemm<kBM, BN>(m - done, n, k, a + done * lda, lda, b, ldb, trans_b, c + done * ldc, ldc, relu, st,
                                     gate ? gate + done * ldg : nullptr, ldg, divisor, out_drop ? &rest_drop : nullptr,
-                                    im.bits ? &rest_mask : nullptr);
+                                    im.bits ? &rest_mask : nullptr, layer ? &rest_layer : nullptr);
     }
     const OutDrop od = out_drop ? out_drop_ready(*out_drop) : OutDrop{0, 1.0f, 0, 0, nullptr, 0, 0};
     const int64_t tiles_m = ceil_div(m, kBM), tiles_n = ceil_div(n, BN);
@@ -937,9 +1022,15 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
     if (n_tiles > INT32_MAX) return fail(GCN_ERR_BAD_ARG, "matrix too large for one launch");
     const int a_vec = (lda % 4 == 0) && (((uintptr_t)a & 15) == 0);
     const int b_vec = (ldb % 4 == 0) && (((uintptr_t)b & 15) == 0);
-#define GCN_GEMM_GO(TB, BK)                                                                                  \
-    gemm_mfma_kernel<kBM, BN, TB, BK><<<(unsigned)n_tiles, kBlock, 0, st>>>(m, n, k, a, lda, b, ldb, c, ldc, relu, a_vec, \
-                                                                       b_vec, tiles_m, tiles_n, gate, ldg, divisor, od, im)
+#define GCN_GEMM_GO(TB, BK)                                                                                         \
+    do {                                                                                                           \
+        if (layer)                                                                                                 \
+            gemm_mfma_kernel<kBM, BN, TB, BK, true><<<(unsigned)n_tiles, kBlock, 0, st>>>(                         \
+                m, n, k, a, lda, b, ldb, c, ldc, relu, a_vec, b_vec, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
+        else                                                                                                       \
+            gemm_mfma_kernel<kBM, BN, TB, BK><<<(unsigned)n_tiles, kBlock, 0, st>>>(                               \
+                m, n, k, a, lda, b, ldb, c, ldc, relu, a_vec, b_vec, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
+    } while (0)
     if (k <= 16) {
         if (trans_b)
             GCN_GEMM_GO(true, 16);
@@ -956,7 +1047,37 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
     return GCN_OK;
 }
 
-// ------------------------------------------------------------------------------------------------
+// A layer's product of few tiles and a long k: the k ranges of the cuts run side by side, at least 64 deep and a multiple
+// of the 32-deep stage, as many as give the chip's 768 workgroup slots one each.
+static int64_t layer_cut_k(int64_t k, int64_t cuts) { return align_up(ceil_div(k, cuts), 32); }
+static int64_t layer_cuts(int64_t m, int64_t n, int64_t k) {
+    if (m == 0 || n == 0 || k < 128) return 1;
+    const int64_t tiles = ceil_div(m, (int64_t)128) * ceil_div(n, (int64_t)(n <= 32 ? 32 : n <= 64 ? 64 : 128));
+    const int64_t cuts = std::min<int64_t>(std::min<int64_t>(768 / tiles, k / 64), 64);
+    return cuts > 1 ? ceil_div(k, layer_cut_k(k, cuts)) : 1;
+}
+
+template <int BN>
+static int launch_cuts(int64_t m, int64_t n, int64_t k, int64_t cuts, const float* a, int64_t lda, const float* b, int64_t ldb,
+                       int trans_b, float* part, hipStream_t st) {
+    const int64_t tiles_m = ceil_div(m, (int64_t)128), tiles_n = ceil_div(n, (int64_t)BN);
+    const int a_vec = (lda % 4 == 0) && (((uintptr_t)a & 15) == 0);
+    const int b_vec = (ldb % 4 == 0) && (((uintptr_t)b & 15) == 0);
+    const OutDrop od = {0, 1.0f, 0, 0, nullptr, 0, 0};
+    const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)cuts);
+    const int64_t k_cut = layer_cut_k(k, cuts);
+#define GCN_CUTS_GO(TB)                                                                                                \
+    gemm_mfma_kernel<128, BN, TB, 32, true><<<grid, kBlock, 0, st>>>(m, n, k, a, lda, b, ldb, part, n, 0, a_vec, b_vec, tiles_m, \
+                                                                     tiles_n, nullptr, 0, 1.0f, od, kNoInMask, kNoEpi, k_cut)
+    if (trans_b)
+        GCN_CUTS_GO(true);
+    else
+        GCN_CUTS_GO(false);
+#undef GCN_CUTS_GO
+    GCN_LAUNCH_CHECK();
+    return GCN_OK;
+}
+
 // ------------------------------------------------------------------------------------------------
 // C[m x n] = act(A[m x k] . B[k x n]) for n <= 32 (hidden -> classes, gcn/layers.py:32-33 on the last layer):
 // A is read once, C is n / k of it, so the product is bound by HBM -- as long as nothing else is in the way.
@@ -1405,6 +1526,43 @@ int gcn_gemm_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, c
     if (n <= 32) return launch_gemm<128, 32>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, relu, st);
     if (n <= 64) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, relu, st);
     return launch_gemm<128, 128>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, relu, st);
+}
+
+int gcn_gemm_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+    if (!bytes || m < 0 || n < 0 || k < 0) return fail(GCN_ERR_BAD_ARG, "bad argument");
+    const int64_t cuts = layer_cuts(m, n, k);
+    *bytes = cuts > 1 ? (size_t)cuts * (size_t)m * (size_t)n * sizeof(float) : 0;
+    return GCN_OK;
+}
+
+int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
+                          int trans_b, const float* bias, int act, const float* residual, int64_t ldr, float* pre,
+                          int64_t ldp, float* c, int64_t ldc, void* workspace, size_t workspace_bytes, void* stream) {
+    if (m < 0 || n < 0 || k < 0) return fail(GCN_ERR_BAD_ARG, "negative dimension");
+    const int64_t most = ((int64_t)1 << 22) - 1;       // byte offsets inside a 128-row tile stay below 2^31
+    if (ldc > most || (residual && ldr > most) || (pre && ldp > most))
+        return fail(GCN_ERR_BAD_ARG, "a leading dimension of the result, the residual or pre is over %lld", (long long)most);
+    if (lda < k || ldc < n || ldb < (trans_b ? k : n) || (residual && ldr < n) || (pre && ldp < n))
+        return fail(GCN_ERR_BAD_ARG, "leading dimension too small");
+    if (act < GCN_ACT_NONE || act > GCN_ACT_SILU) return fail(GCN_ERR_BAD_ARG, "unknown activation %d", act);
+    if (m == 0 || n == 0) return GCN_OK;
+    if (!c || (k > 0 && (!a || !b))) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    const EpiArgs ep = {bias, residual, residual ? ldr : 0, pre, pre ? ldp : 0, act};
+    const int64_t cuts = layer_cuts(m, n, k);
+    if (cuts > 1) {
+        const size_t need = (size_t)cuts * (size_t)m * (size_t)n * sizeof(float);
+        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+            return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
+        if (int rc = n <= 32   ? launch_cuts<32>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)
+                     : n <= 64 ? launch_cuts<64>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)
+                               : launch_cuts<128>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st))
+            return rc;
+        return launch_join_splits(m, n, cuts, (const float*)workspace, ep, c, ldc, st);
+    }
+    if (n <= 32) return launch_gemm<128, 32>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
+    if (n <= 64) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
+    return launch_gemm<128, 128>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
 }
 
 int gcn_gemm_gated_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,

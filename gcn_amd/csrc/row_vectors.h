@@ -37,4 +37,7 @@ __device__ __forceinline__ void store_cols(float* __restrict__ row, int c, int f
     }
 }
 
+// out[c] = sum over the rows of part [rows x f], in a fixed order (norm.hip)
+int launch_column_sums(int64_t rows, int64_t f, const float* part, float* out, hipStream_t st);
+
 }  // namespace gcn

@@ -1076,6 +1076,78 @@ def spmm_quant(a, q, relu=False, out=None):
 
 
 # --------------------------------------------------------------------------- #
+# dense layer: product with bias, activation and residual in its store
+# --------------------------------------------------------------------------- #
+_ACTS = {None: _lib.GCN_ACT_NONE, 'none': _lib.GCN_ACT_NONE, 'relu': _lib.GCN_ACT_RELU, 'gelu': _lib.GCN_ACT_GELU,
+         'silu': _lib.GCN_ACT_SILU}
+
+
+def _act_code(act):
+    if act not in _ACTS:
+        raise ValueError('unknown activation %r: one of %s' % (act, sorted(k for k in _ACTS if k)))
+    return _ACTS[act]
+
+
+def gemm_epilogue(a, b, trans_b=False, bias=None, act=None, residual=None, out=None, want_pre=False):
+    """``act(a @ b + bias) + residual`` (``a @ b.T`` with ``trans_b``) in one product; ``act``: None, 'relu', 'gelu' (the
+    normal distribution function, no tanh) or 'silu'.  ``residual`` may be ``out`` itself.  With ``want_pre`` returns
+    ``(result, pre)``, ``pre = a @ b + bias`` as ``act_grad`` wants it."""
+    code = _act_code(act)
+    with _on_device(a, b, bias, residual, out):
+        a, b = _rowmajor(a), _rowmajor(b)
+        m, k = a.shape
+        n = b.shape[0] if trans_b else b.shape[1]
+        if (b.shape[1] if trans_b else b.shape[0]) != k:
+            raise ValueError('shape mismatch in gemm_epilogue')
+        bias = _vector(bias, n, 'the bias')
+        if residual is not None:
+            residual = _rowmajor(residual)
+            if tuple(residual.shape) != (m, n):
+                raise ValueError('the residual must have the shape of the result')
+        if out is None:
+            c = torch.empty((m, n), dtype=torch.float32, device=a.device)
+        else:
+            _check_out(out, m, n)
+            c = out
+        pre = torch.empty((m, n), dtype=torch.float32, device=a.device) if want_pre else None
+        need, ws = ctypes.c_size_t(), None
+        _lib.call('gcn_gemm_epilogue_workspace_bytes', m, n, k, ctypes.byref(need))
+        if need.value:
+            ws = _workspace(need.value, a.device)
+        _lib.call('gcn_gemm_epilogue_f32', m, n, k, _p(a), _ld(a), _p(b), _ld(b), 1 if trans_b else 0, _p(bias), code,
+                  _p(residual), 0 if residual is None else _ld(residual), _p(pre), n, _p(c), _ld(c), _p(ws), need.value,
+                  _stream())
+    return (c, pre) if want_pre else c
+
+
+def act_grad(grad, pre, act, want_bias=True):
+    """``(dz, dbias)`` of ``gemm_epilogue``: ``dz = grad * act'(pre)`` (``grad`` itself without an activation) and its sum
+    over the rows, in a fixed order (None without ``want_bias``).  The other gradients are ``gemm(dz, b, trans_b=True)``,
+    ``gemm_tn(a, dz)`` and, for the residual, ``grad``."""
+    code = _act_code(act)
+    with _on_device(grad, pre):
+        grad = _rowmajor(grad)
+        m, n = grad.shape
+        if code != _lib.GCN_ACT_NONE:
+            if pre is None:
+                raise ValueError('the gradient of an activation wants the pre-activation')
+            pre = _rowmajor(pre)
+            if pre.shape != grad.shape:
+                raise ValueError('the pre-activation has another shape than the gradient')
+            dz = torch.empty((m, n), dtype=torch.float32, device=grad.device)
+        else:
+            pre, dz = None, None
+        dbias, ws, need = None, None, ctypes.c_size_t()
+        if want_bias:
+            dbias = torch.empty(n, dtype=torch.float32, device=grad.device)
+            _lib.call('gcn_act_grad_workspace_bytes', m, n, ctypes.byref(need))
+            ws = _workspace(need.value, grad.device)
+        _lib.call('gcn_act_grad_f32', m, n, code, _p(grad), _ld(grad), _p(pre), 0 if pre is None else _ld(pre), _p(dz), n,
+                  _p(dbias), _p(ws), need.value, _stream())
+    return (grad if dz is None else dz), dbias
+
+
+# --------------------------------------------------------------------------- #
 # distillation
 # --------------------------------------------------------------------------- #
 _VALUE_TYPES = {torch.float32: _lib.GCN_F32, torch.float16: _lib.GCN_F16, torch.bfloat16: _lib.GCN_BF16}

@@ -45,6 +45,11 @@ typedef enum {
 #define GCN_RELU 1            /* act = relu fused into the epilogue                  (gcn/layers.py:214, models.py:17) */
 #define GCN_SPLIT_WIDE 4      /* spmm: cut long rows every 1024 entries whatever the width, so that a product
                                  computed over ranges of feature columns equals the full-width one bit for bit */
+/* activations of a dense layer's epilogue */
+#define GCN_ACT_NONE 0
+#define GCN_ACT_RELU 1
+#define GCN_ACT_GELU 2        /* z * Phi(z), Phi the normal distribution function (no tanh approximation) */
+#define GCN_ACT_SILU 3        /* z / (1 + e^-z) */
 /* element types of stored values */
 #define GCN_F32 0
 #define GCN_F16 1
@@ -560,6 +565,24 @@ int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, c
 int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, const int32_t* indices, const float* vals,
                            int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* c, int64_t ldc, int flags,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* C[m x n] = act(A . op(B) + bias) + residual: gcn_gemm_f32 (tf.matmul, gcn/layers.py:32-33) with a dense layer's
+ * epilogue in its store.  bias [n], residual [m x n] (may be C itself) and pre may be NULL; pre [m x n] receives the
+ * pre-activation A . op(B) + bias, which gcn_act_grad_f32 wants.  A product of few tiles and a long k is cut along k, the
+ * cuts' partial products go to the workspace and are added in order; query its size first (0 when one cut is enough;
+ * 16-byte aligned).  ldc, ldr and ldp are at most 2^22 - 1. */
+int gcn_gemm_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
+                          int trans_b, const float* bias, int act, const float* residual, int64_t ldr, float* pre,
+                          int64_t ldp, float* c, int64_t ldc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The part of its backward pass that is no product: dz = dout * act'(pre) (may be dout itself; NULL: not wanted) and
+ * dbias [n] (may be NULL) = the sum of dz over the rows, in a fixed order.  pre is not read for GCN_ACT_NONE.  The gradients
+ * of A, B and the residual are gcn_gemm_f32 (trans_b swapped) and gcn_gemm_tn_f32 on dz, and dout.  Workspace (16-byte
+ * aligned) as the query says, not needed without dbias. */
+int gcn_act_grad_workspace_bytes(int64_t m, int64_t n, size_t* bytes);
+int gcn_act_grad_f32(int64_t m, int64_t n, int act, const float* dout, int64_t ldo, const float* pre, int64_t ldp, float* dz,
+                     int64_t ldz, float* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Distillation from a teacher's top logits under the reference's mask (gcn/metrics.py:85-92), with the gradient
  * optimizer.minimize (gcn/models.py:86) would derive.  Row i lists k <= 256 teacher logits (value_type GCN_F32, GCN_F16 or

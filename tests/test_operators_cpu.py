@@ -1,4 +1,5 @@
-"""CPU: the argument checks of the row norm and the distillation loss through the C ABI -- they return before any HIP call -- and what the
+"""CPU: the argument checks of the row norm, the 8-bit product, the dense epilogue and the
+distillation loss through the C ABI -- they return before any HIP call -- and what the
 Python operators refuse on a host without a GPU."""
 import ctypes
 
@@ -68,6 +69,44 @@ def test_distillation_refuses():
         assert _distill(**bad) == BAD, bad
 
 
+def _dense(m=4, n=5, k=6, a=P, lda=6, b=P, ldb=5, tb=0, bias=P, act=1, r=P, ldr=5, pre=P, ldp=5, c=P, ldc=5, ws=None, nb=0):
+    return _lib().gcn_gemm_epilogue_f32(m, n, k, a, lda, b, ldb, tb, bias, act, r, ldr, pre, ldp, c, ldc, ws, nb, None)
+
+
+def test_dense_epilogue_refuses():
+    assert _dense(m=0) == 0 and _dense(n=0, ldb=0) == 0
+    for bad in (dict(m=-1), dict(n=-1), dict(k=-1), dict(lda=5), dict(ldb=4), dict(ldc=4), dict(ldr=4), dict(ldp=4),
+                dict(tb=1, ldb=5), dict(act=-1), dict(act=4), dict(a=None), dict(b=None), dict(c=None), dict(ldc=1 << 22),
+                dict(ldr=1 << 22), dict(ldp=1 << 22)):
+        assert _dense(**bad) == BAD, bad
+    need = ctypes.c_size_t()
+    assert _lib().gcn_gemm_epilogue_workspace_bytes(128, 16, 2048, ctypes.byref(need)) == 0 and need.value > 0
+    long = dict(m=128, n=16, k=2048, lda=2048, ldb=16, ldc=16, ldr=16, ldp=16)
+    for bad in (dict(ws=None, nb=need.value), dict(ws=P, nb=need.value - 1), dict(ws=P + 4, nb=need.value)):
+        assert _dense(**long, **bad) == WORKSPACE, bad
+    assert _lib().gcn_gemm_epilogue_workspace_bytes(1 << 20, 256, 256, ctypes.byref(need)) == 0 and need.value == 0
+    assert _lib().gcn_gemm_epilogue_workspace_bytes(-1, 1, 1, ctypes.byref(need)) == BAD
+
+
+def _act_grad(m=4, n=5, act=2, g=P, ldo=5, pre=P, ldp=5, dz=P, ldz=5, db=None, ws=None, nb=0):
+    return _lib().gcn_act_grad_f32(m, n, act, g, ldo, pre, ldp, dz, ldz, db, ws, nb, None)
+
+
+def test_activation_gradient_refuses():
+    assert _act_grad(m=0) == 0 and _act_grad(n=0) == 0 and _act_grad(dz=None) == 0
+    for bad in (dict(m=-1), dict(n=-1), dict(act=9), dict(ldo=4), dict(ldp=4), dict(ldz=4), dict(g=None), dict(pre=None)):
+        assert _act_grad(**bad) == BAD, bad
+    need = ctypes.c_size_t()
+    assert _lib().gcn_act_grad_workspace_bytes(4, 5, ctypes.byref(need)) == 0 and need.value >= 20
+    for bad in (dict(ws=None, nb=need.value), dict(ws=P, nb=need.value - 1), dict(ws=P + 8, nb=need.value)):
+        assert _act_grad(db=P, **bad) == WORKSPACE, bad
+
+
+def test_quant_product_refuses():
+    lib = _lib()
+    assert lib.gcn_spmm_csr_quant_f32(None, P, P, P, 4, P, 16, P, P, 4, 0, None, 0, None) == BAD
+
+
 def test_host_tensors_are_refused():
     import torch
     from gcn_amd import sparse
@@ -75,6 +114,7 @@ def test_host_tensors_are_refused():
         pytest.skip('host-only check')
     x = torch.ones(2, 4)
     for call in (lambda: sparse.rms_norm(x), lambda: sparse.rms_norm_grad(x, x, None, torch.ones(2)),
+                 lambda: sparse.gemm_epilogue(x, x, trans_b=True), lambda: sparse.act_grad(x, x, 'relu'),
                  lambda: sparse.distill_topk(x, x, x.int(), None, 1.0), lambda: sparse.QuantRows(2, 4, torch.zeros((2, 16), dtype=torch.uint8), torch.ones(2))):
         with pytest.raises(ValueError):
             call()
