@@ -5,6 +5,7 @@ names and defaults.  Every product runs in ``libgcn_hip.so``; torch supplies mem
 and the autograd tape.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import graph, inits, sparse
 
@@ -144,6 +145,102 @@ class _GatedGemmFn(torch.autograd.Function):
         return d_h, d_w, None
 
 
+def _accumulators(*inputs):
+    """The gradient accumulators of the leaves among the inputs, to be held over the call that uses them.  Refuses to record
+    a differentiable call while an eager graph over the same leaves lives: such a graph keeps the accumulators, which
+    belong to the stream it was built on, and a backward pass recorded over them waits for
+    that stream, which ends the capture and the process.  Eager calls mark the accumulators; a mark dies with the
+    accumulator, that is, with the last eager graph over the leaf."""
+    held = []
+    if not torch.is_grad_enabled():
+        return held
+    capturing = torch.cuda.is_current_stream_capturing()
+    for t in inputs:
+        if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf:
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            if not capturing:
+                node.metadata['gcn_amd_eager'] = True
+            elif node.metadata.get('gcn_amd_eager'):
+                raise RuntimeError('an eager autograd graph over an input of this recorded call is alive: drop its outputs '
+                                   'and losses before capturing')
+            held.append(node)
+    return held
+
+
+class _RmsNormFn(torch.autograd.Function):
+    """(y, h) = rms norm of h = x + residual (y alone without a residual); h and the rows' 1 / rms are kept."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, inv = sparse.rms_norm(x, weight, residual=residual, eps=eps)
+        ctx.save_for_backward(h, weight, inv)
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_h=None):
+        h, weight, inv = ctx.saved_tensors
+        dx, dw = _norm_grads(grad, grad_h, h, weight, inv, ctx.needs_input_grad[1])
+        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+
+
+def _norm_grads(grad, grad_h, h, weight, inv, want_weight):
+    if grad is None:
+        return grad_h, torch.zeros_like(weight) if want_weight else None
+    return sparse.rms_norm_grad(grad, h, weight, inv, grad_h=grad_h, want_weight=want_weight)
+
+
+class _QuantDotFn(torch.autograd.Function):
+    """(out, h) = act(A . e4m3 rows of the norm of h = x + residual); backward: the gradient goes through the rounding to
+    8 bits unchanged (the product's gradient is that of the values the rows stand for), dy = A^T . dOut in float32."""
+
+    @staticmethod
+    def forward(ctx, support, x, weight, residual, eps, relu):
+        q, h, inv = sparse.rms_norm(x, weight, residual=residual, eps=eps, quant=True)
+        out = sparse.spmm_quant(support, q, relu=relu)
+        ctx.support, ctx.relu = support, relu
+        ctx.save_for_backward(h, weight, inv, out if relu else None)
+        ctx.set_materialize_grads(False)
+        return out if residual is None else (out, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_h=None):
+        h, weight, inv, out = ctx.saved_tensors
+        if grad is not None:
+            if ctx.relu:
+                grad = sparse.dropout(grad, 1.0, 0, 0, gate=out)
+            grad = sparse.spmm(ctx.support.transpose(), grad)
+        dx, dw = _norm_grads(grad, grad_h, h, weight, inv, ctx.needs_input_grad[2])
+        return None, dx, dw, dx if ctx.needs_input_grad[3] else None, None, None
+
+
+class _DenseFn(torch.autograd.Function):
+    """act(x . w + bias) + residual in one product; the pre-activation is kept for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual):
+        keep = any(ctx.needs_input_grad) and act not in (None, 'none')
+        out = sparse.gemm_epilogue(x, w, bias=bias, act=act, residual=residual, want_pre=keep)
+        out, pre = out if keep else (out, None)
+        ctx.act = act
+        ctx.save_for_backward(x, w, pre)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, w, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = dbias = None
+        if need[0] or need[1] or need[2]:
+            dz, dbias = sparse.act_grad(grad, pre, ctx.act, want_bias=need[2])
+            dx = sparse.gemm(dz, w, trans_b=True) if need[0] else None
+            dw = sparse.gemm_tn(x, dz) if need[1] else None
+        return dx, dw, dbias, None, grad if need[4] else None
+
+
 class DroppedSparse(object):
     """A sparse matrix with a pending ``sparse_dropout``: the mask is applied inside the next product."""
 
@@ -193,6 +290,31 @@ def dot(x, y, sparse=False, fuse_relu=False, out_dropout=None, dropped_input=Non
         return _SpmmFn.apply(x, y, fuse_relu, out_dropout if fuse_relu else None)
     res = _GatedGemmFn.apply(x, y, dropped_input) if dropped_input is not None else _GemmFn.apply(x, y)
     return torch.relu(res) if fuse_relu else res
+
+
+# --------------------------------------------------------------------------- #
+# pieces of deeper layers (no counterpart in the reference)
+# --------------------------------------------------------------------------- #
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """The rows of ``h = x + residual`` over their root mean square, times ``weight``: returns ``y``, or ``(y, h)`` with a
+    residual -- ``h`` is what the next layer adds.  Differentiable in x, weight and residual."""
+    held = _accumulators(x, weight, residual)        # noqa: F841 -- alive until the call below has its graph
+    return _RmsNormFn.apply(x, weight, residual, float(eps))
+
+
+def quant_dot(support, x, weight=None, residual=None, eps=1e-6, fuse_relu=False):
+    """``dot(support, rms_norm(x, ...), sparse=True)`` with the normalised rows in 8 bits (a scale a row): the product
+    gathers a quarter of the bytes.  Returns ``out``, or ``(out, h)`` with a residual.  Differentiable in x, weight and
+    residual; the rounding to 8 bits passes the gradient on unchanged."""
+    held = _accumulators(x, weight, residual)        # noqa: F841 -- alive until the call below has its graph
+    return _QuantDotFn.apply(support, x, weight, residual, float(eps), bool(fuse_relu))
+
+
+def dense(x, w, bias=None, act=None, residual=None):
+    """``act(x @ w + bias) + residual`` in one product; ``act``: None, 'relu', 'gelu' or 'silu'.  Differentiable in every
+    tensor."""
+    held = _accumulators(x, w, bias, residual)        # noqa: F841 -- alive until the call below has its graph
+    return _DenseFn.apply(x, w, bias, act, residual)
 
 
 # --------------------------------------------------------------------------- #

@@ -118,3 +118,23 @@ def test_host_tensors_are_refused():
                  lambda: sparse.distill_topk(x, x, x.int(), None, 1.0), lambda: sparse.QuantRows(2, 4, torch.zeros((2, 16), dtype=torch.uint8), torch.ones(2))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_recording_over_a_live_eager_graph_is_refused(monkeypatch):
+    """The check marks a leaf's accumulator in eager calls; the mark lives as long as a graph holds the accumulator."""
+    import torch
+    from gcn_amd import layers
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: capturing[0])
+    leaf = torch.ones(3, requires_grad=True)
+    nodes = layers._accumulators(leaf, None, torch.ones(2))
+    assert len(nodes) == 1
+    held = (leaf * 2).sum()                       # what a wrapper's call does while it holds the nodes
+    del nodes
+    capturing[0] = True
+    with pytest.raises(RuntimeError):
+        layers._accumulators(leaf)
+    with torch.no_grad():
+        assert layers._accumulators(leaf) == []
+    del held
+    assert len(layers._accumulators(leaf)) == 1
