@@ -172,7 +172,7 @@ __global__ void gather_rows_kernel(int64_t n_out, int64_t f, const float* __rest
 //    consecutive k with one ds_read_b128.  B uses the same k mapping, which makes every step an
 //    exact rank-2 update; only the order in which the 32 products of a stage are added differs
 //    from ascending k.
-//  - Interior blocks (whole tile in range, 16-byte aligned rows) run a main loop without any bounds
+//  - Interior blocks (whole tile in range) run a main loop without any bounds
 //    test: a guarded load is a branch per element, and branches between the loads and the MFMAs
 //    keep the compiler from overlapping them (85 -> 121 TFLOP/s on 2^22 x 512 x 512).  The last
 //    partial k tile and edge blocks take the guarded loader.
@@ -180,6 +180,13 @@ __global__ void gather_rows_kernel(int64_t n_out, int64_t f, const float* __rest
 //    tiles of one row panel one after the other.
 // ------------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float quad_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// four consecutive floats at any 4-byte aligned address: the hardware's 128-bit load wants no more than that
+__device__ __forceinline__ float4 load_quad(const float* p) {
+    const quad_any t = *reinterpret_cast<const quad_any*>(p);
+    return make_float4(t.x, t.y, t.z, t.w);
+}
 
 // The store of a dense layer's tile: C = act(acc + bias) + residual, the pre-activation to pre.  Every access is a buffer
 // instruction on a range that ends with the tile's last element, and the lanes of columns past n point behind it: the
@@ -217,7 +224,7 @@ __device__ __forceinline__ void store_layer_tile(const f32x16 (&acc)[MT][NT], co
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int row = i * 32 + (e & 3) + 8 * (e >> 2);
-                    const float z = acc[i][j][e] + add;
+                    const float z = ep.bias ? acc[i][j][e] + add : acc[i][j][e];      // without a bias -0 stays -0
                     if (ep.pre)
                         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(z), res_p,
                                                               (int)(at_p + (uint32_t)(row * (int)ep.ldp) * 4u), 0, 0);
@@ -238,8 +245,8 @@ template <int kBM, int BN, bool TRANS_B, int kBK, bool LAYER = false>
 __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t n, int64_t k,
                                                            const float* __restrict__ a, int64_t lda,
                                                            const float* __restrict__ b, int64_t ldb,
-                                                           float* __restrict__ c, int64_t ldc, int relu, int a_vec,
-                                                           int b_vec, int64_t tiles_m, int64_t tiles_n,
+                                                           float* __restrict__ c, int64_t ldc, int relu,
+                                                           int64_t tiles_m, int64_t tiles_n,
                                                            const float* __restrict__ gate, int64_t ldg,
                                                            float divisor, OutDrop od, InMask im, EpiArgs ep,
                                                            int64_t k_cut) {
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
     auto load_a_fast = [&](int64_t k0) {
 #pragma unroll
         for (int i = 0; i < kAPer; ++i) {
-            ra[i] = *reinterpret_cast<const float4*>(a + (m0 + a_r + kARows * i) * lda + k0 + a_kq);
+            ra[i] = load_quad(a + (m0 + a_r + kARows * i) * lda + k0 + a_kq);
             mask_a(i, m0 + a_r + kARows * i, k0);
         }
     };
@@ -319,9 +326,9 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             const int u = tid + kBlock * p;
             if (!kBAll && u >= kBUnits) continue;
             if (TRANS_B)
-                rb[p] = *reinterpret_cast<const float4*>(b + (n0 + u / kKQ) * ldb + k0 + (u % kKQ) * 4);
+                rb[p] = load_quad(b + (n0 + u / kKQ) * ldb + k0 + (u % kKQ) * 4);
             else
-                rb[p] = *reinterpret_cast<const float4*>(b + (k0 + u / (BN / 4)) * ldb + n0 + (u % (BN / 4)) * 4);
+                rb[p] = load_quad(b + (k0 + u / (BN / 4)) * ldb + n0 + (u % (BN / 4)) * 4);
         }
     };
     auto load_a_guarded = [&](int64_t k0) {
@@ -329,8 +336,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
         for (int i = 0; i < kAPer; ++i) {
             const int64_t gr = m0 + a_r + kARows * i;
             const float* ap = a + gr * lda + k0 + a_kq;
-            if (gr < m && a_vec && k0 + a_kq + 4 <= k) {
-                ra[i] = *reinterpret_cast<const float4*>(ap);
+            if (gr < m && k0 + a_kq + 4 <= k) {
+                ra[i] = load_quad(ap);
             } else {
                 float t[4];
 #pragma unroll
@@ -350,8 +357,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
                 const int64_t gc = n0 + u / kKQ;
                 const int kq = (u % kKQ) * 4;
                 const float* bp = b + gc * ldb + k0 + kq;
-                if (gc < n && b_vec && k0 + kq + 4 <= k) {
-                    rb[p] = *reinterpret_cast<const float4*>(bp);
+                if (gc < n && k0 + kq + 4 <= k) {
+                    rb[p] = load_quad(bp);
                     continue;
                 }
 #pragma unroll
@@ -359,8 +366,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             } else {
                 const int64_t gk = k0 + u / (BN / 4), gc = n0 + (u % (BN / 4)) * 4;
                 const float* bp = b + gk * ldb + gc;
-                if (gk < k && b_vec && gc + 4 <= n) {
-                    rb[p] = *reinterpret_cast<const float4*>(bp);
+                if (gk < k && gc + 4 <= n) {
+                    rb[p] = load_quad(bp);
                     continue;
                 }
 #pragma unroll
@@ -429,8 +436,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
     };
 
     const int64_t n_ktiles = (k + kBK - 1) / kBK;
-    const bool a_inside = (m0 + kBM <= m) && a_vec;      // the A tile needs no guards (full k tiles)
-    const bool b_inside = (n0 + BN <= n) && b_vec;
+    const bool a_inside = m0 + kBM <= m;      // the A tile needs no guards (full k tiles)
+    const bool b_inside = n0 + BN <= n;
     const bool interior = (m0 + kBM <= m) && (n0 + BN <= n);
     const int64_t n_full = a_inside ? k / kBK : 0;       // leading k tiles whose A loads need no guards
     if (n_ktiles > 0) {
@@ -645,14 +652,19 @@ __device__ __forceinline__ uint32_t quad_read(uint32_t x, int src) {
     }
 }
 
-template <bool TRANS_B, int EPI, bool A_MASK = false>
+// RAGGED (EPI == kEpiLayer): any m, n and k and any alignment.  Rows of A past the end (and columns of B past n) repeat
+// the last one -- what they give is not stored --, and the last 1 to 32 of k, loaded element by element with zeros
+// past the end, come after n_ktiles whole stages: every address lies inside the operands, and the main loop has no test.
+// The guarded kernel ran 150,001 x 500 x 256 at 103 TFLOP/s, this one at 109, and its gradient
+// 150,001 x 256 x 500 (B [n x k]) at 113 instead of 97.  Same order of additions.
+template <bool TRANS_B, int EPI, bool A_MASK = false, bool RAGGED = false>
 __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int n_ktiles,
                                                                const float* __restrict__ a, int64_t lda,
                                                                const float* __restrict__ b, int64_t ldb,
                                                                float* __restrict__ c, int64_t ldc, int relu,
                                                                const float* __restrict__ gate, int64_t ldg,
                                                                float divisor, InMask im, OutDrop od, int raster,
-                                                               EpiArgs ep) {
+                                                               EpiArgs ep, int64_t m, int64_t n, int k) {
     constexpr int kBM = 128, BN = 128, kBK = 32, MT = 2, NT = 2;
     constexpr int kAPitch = kBK + 4, kBPitch = BN + 4;
     __shared__ __attribute__((aligned(16))) float as[kBM * kAPitch];
@@ -691,6 +703,17 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
     // B [n x k]: column tid / 8 + 32 p, k quad tid % 8.
     const int a_voff = ((tid >> 3) * (int)lda + (tid & 7) * 4) * 4;
     const int b_voff = TRANS_B ? ((tid >> 3) * (int)ldb + (tid & 7) * 4) * 4 : ((tid >> 5) * (int)ldb + (tid & 31) * 4) * 4;
+    const int m_left = RAGGED ? (int)(m - m0 < kBM ? m - m0 : kBM) : kBM, n_left = RAGGED ? (int)(n - n0 < BN ? n - n0 : BN) : BN;
+    // RAGGED: byte offsets of the thread's four rows of A (and columns of B [n x k]); of its column quad of B [k x n]
+    int a_row[4], b_row[4];
+    if (RAGGED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a_row[i] = min((tid >> 3) + 32 * i, m_left - 1) * (int)lda * 4;
+            b_row[i] = TRANS_B ? min((tid >> 3) + 32 * i, n_left - 1) * (int)ldb * 4
+                               : ((tid >> 5) * (int)ldb + ((tid & 31) * 4 < n_left ? (tid & 31) * 4 : 0)) * 4;
+        }
+    }
     const int a_step = 32 * (int)lda * 4;                                   // unit i -> i + 1
     const int b_step = TRANS_B ? 32 * (int)ldb * 4 : 8 * (int)ldb * 4;       // unit p -> p + 1
     const int b_kstep = TRANS_B ? kBK * 4 : kBK * (int)ldb * 4;              // one k stage
@@ -705,14 +728,17 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const f32x4v v = __builtin_bit_cast(
-                f32x4v, __builtin_amdgcn_raw_buffer_load_b128(res_a, a_voff, a_k + i * a_step, 0));
+                f32x4v, RAGGED ? __builtin_amdgcn_raw_buffer_load_b128(res_a, a_row[i] + (tid & 7) * 16, a_k, 0)
+                               : __builtin_amdgcn_raw_buffer_load_b128(res_a, a_voff, a_k + i * a_step, 0));
             ra[i] = make_float4(v.x, v.y, v.z, v.w);
             if (A_MASK) rm[i] = __builtin_amdgcn_raw_buffer_load_b32(res_m, m_voff, (a_k >> 5) + i * m_step, 0);
         }
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             const f32x4v v = __builtin_bit_cast(
-                f32x4v, __builtin_amdgcn_raw_buffer_load_b128(res_b, b_voff, b_k + p * b_step, 0));
+                f32x4v, RAGGED && TRANS_B ? __builtin_amdgcn_raw_buffer_load_b128(res_b, b_row[p] + (tid & 7) * 16, b_k, 0)
+                                          : __builtin_amdgcn_raw_buffer_load_b128(res_b, RAGGED ? b_row[p] : b_voff,
+                                                                                  b_k + p * b_step, 0));
             rb[p] = make_float4(v.x, v.y, v.z, v.w);
         }
     };
@@ -784,10 +810,53 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
         }
     };
 
+    // the last stage of a ragged k: elements past the end are zero, their addresses those of the last one
+    auto load_tail = [&](int k0) {
+        auto one = [&](const __amdgpu_buffer_rsrc_t& res, int offset, bool in) {
+            const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(res, offset, 0, 0));
+            return in ? v : 0.0f;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int kk = k0 + (tid & 7) * 4 + e;
+                x[e] = one(res_a, a_row[i] + min(kk, k - 1) * 4, kk < k);
+                if (TRANS_B) {
+                    y[e] = one(res_b, b_row[i] + min(kk, k - 1) * 4, kk < k);
+                } else {
+                    const int kr = k0 + (tid >> 5) + 8 * i, col = (tid & 31) * 4 + e;
+                    y[e] = one(res_b, (min(kr, k - 1) * (int)ldb + min(col, n_left - 1)) * 4, kr < k);
+                }
+            }
+            ra[i] = make_float4(x[0], x[1], x[2], x[3]);
+            rb[i] = make_float4(y[0], y[1], y[2], y[3]);
+        }
+    };
+
     load_stage(0, 0);
     store_tile();
     __syncthreads();
-    if (n_ktiles == 1) {
+    if (RAGGED) {
+        int a_k = 0, b_k = 0;
+        for (int t = 1; t <= n_ktiles; ++t) {
+            a_k += kBK * 4;
+            b_k += b_kstep;
+            if (t < n_ktiles)
+                load_stage(a_k, b_k);
+            else
+                load_tail(t * kBK);
+            if (t == 1)
+                compute(std::true_type{});
+            else
+                compute(std::false_type{});
+            __syncthreads();
+            store_tile();
+            __syncthreads();
+        }
+        compute(std::false_type{});
+    } else if (n_ktiles == 1) {
         compute(std::true_type{});
     } else {
         int a_k = kBK * 4, b_k = b_kstep;
@@ -850,7 +919,7 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
         return;
     }
     if (EPI == kEpiLayer) {
-        store_layer_tile<MT, NT>(acc, ep, c, ldc, m0, n0, kBM, BN, wm * MT * 32, wn * NT * 32, lane);
+        store_layer_tile<MT, NT>(acc, ep, c, ldc, m0, n0, m_left, n_left, wm * MT * 32, wn * NT * 32, lane);
         return;
     }
     if (EPI == kEpiDrop) {
@@ -949,6 +1018,15 @@ static bool panels_form_fits(int64_t m, int64_t n, int64_t k, const float* a, in
     return m / 128 <= 8 * 65535;
 }
 
+// true when the ragged form of gemm_panels_kernel takes the problem: byte offsets inside a tile's operands and its output
+// below 2^31 (the output's leading dimensions as store_layer_tile wants them)
+static bool ragged_form_fits(int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int trans_b, int64_t ldc) {
+    const int64_t limit = (int64_t)1 << 29;
+    if (k <= 32 || n <= 64 || ldc >= (int64_t)1 << 22 || k + 32 >= limit) return false;
+    if (128 * lda + k >= limit || (trans_b ? 128 * ldb + k >= limit : (k + 32) * ldb + 128 >= limit)) return false;
+    return m <= (int64_t)8 * 65535 * 128 && ceil_div(n, (int64_t)128) <= (1 << 20);
+}
+
 static const InMask kNoInMask = {nullptr, 0, 1.0f, 1.0f, 1};
 static const EpiArgs kNoEpi = {nullptr, nullptr, 0, nullptr, 0, GCN_ACT_NONE};
 
@@ -971,7 +1049,7 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
         const int raster = n / 128 >= 16 ? 1 : 0;
 #define GCN_PANELS_GO(TB, EPI, AM)                                                                                \
     gemm_panels_kernel<TB, EPI, AM><<<grid, kBlock, 0, st>>>((int)panels, (int)(k / 32), a, lda, b, ldb, c, ldc, relu, gate, \
-                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster, ep)
+                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster, ep, m, n, (int)k)
         if (im.bits) {
             GCN_PANELS_GO(false, kEpiPlain, true);
         } else if (layer) {
@@ -1016,20 +1094,36 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
                                     gate ? gate + done * ldg : nullptr, ldg, divisor, out_drop ? &rest_drop : nullptr,
                                     im.bits ? &rest_mask : nullptr, layer ? &rest_layer : nullptr);
     }
+    // the plain product and the layer's epilogue of every other shape with more than one stage of k: whole and ragged
+    // panels alike through the kernel whose main loop has no guards (the guarded kernel keeps the other epilogues, the
+    // ReLU whose store maps NaN to 0, and pitches past 32-bit offsets)
+    if (kBM == 128 && BN == 128 && !im.bits && !out_drop && !gate && !relu && ragged_form_fits(m, n, k, lda, ldb, trans_b, ldc)) {
+        const int64_t panels = ceil_div(m, (int64_t)128), col_tiles = ceil_div(n, (int64_t)128);
+        const dim3 grid((unsigned)(8 * col_tiles), (unsigned)ceil_div(panels, (int64_t)8));
+#define GCN_RAGGED_GO(TB)                                                                                           \
+    gemm_panels_kernel<TB, kEpiLayer, false, true><<<grid, kBlock, 0, st>>>(                                        \
+        (int)panels, (int)((k - 1) / 32), a, lda, b, ldb, c, ldc, 0, nullptr, 0, 1.0f, kNoInMask, no_drop, col_tiles >= 16, ep, m, \
+        n, (int)k)
+        if (trans_b)
+            GCN_RAGGED_GO(true);
+        else
+            GCN_RAGGED_GO(false);
+#undef GCN_RAGGED_GO
+        GCN_LAUNCH_CHECK();
+        return GCN_OK;
+    }
     const OutDrop od = out_drop ? out_drop_ready(*out_drop) : OutDrop{0, 1.0f, 0, 0, nullptr, 0, 0};
     const int64_t tiles_m = ceil_div(m, kBM), tiles_n = ceil_div(n, BN);
     const int64_t n_tiles = tiles_m * tiles_n;
     if (n_tiles > INT32_MAX) return fail(GCN_ERR_BAD_ARG, "matrix too large for one launch");
-    const int a_vec = (lda % 4 == 0) && (((uintptr_t)a & 15) == 0);
-    const int b_vec = (ldb % 4 == 0) && (((uintptr_t)b & 15) == 0);
 #define GCN_GEMM_GO(TB, BK)                                                                                         \
     do {                                                                                                           \
         if (layer)                                                                                                 \
             gemm_mfma_kernel<kBM, BN, TB, BK, true><<<(unsigned)n_tiles, kBlock, 0, st>>>(                         \
-                m, n, k, a, lda, b, ldb, c, ldc, relu, a_vec, b_vec, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
+                m, n, k, a, lda, b, ldb, c, ldc, relu, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
         else                                                                                                       \
             gemm_mfma_kernel<kBM, BN, TB, BK><<<(unsigned)n_tiles, kBlock, 0, st>>>(                               \
-                m, n, k, a, lda, b, ldb, c, ldc, relu, a_vec, b_vec, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
+                m, n, k, a, lda, b, ldb, c, ldc, relu, tiles_m, tiles_n, gate, ldg, divisor, od, im, ep, 0); \
     } while (0)
     if (k <= 16) {
         if (trans_b)
@@ -1061,13 +1155,11 @@ template <int BN>
 static int launch_cuts(int64_t m, int64_t n, int64_t k, int64_t cuts, const float* a, int64_t lda, const float* b, int64_t ldb,
                        int trans_b, float* part, hipStream_t st) {
     const int64_t tiles_m = ceil_div(m, (int64_t)128), tiles_n = ceil_div(n, (int64_t)BN);
-    const int a_vec = (lda % 4 == 0) && (((uintptr_t)a & 15) == 0);
-    const int b_vec = (ldb % 4 == 0) && (((uintptr_t)b & 15) == 0);
     const OutDrop od = {0, 1.0f, 0, 0, nullptr, 0, 0};
     const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)cuts);
     const int64_t k_cut = layer_cut_k(k, cuts);
 #define GCN_CUTS_GO(TB)                                                                                                \
-    gemm_mfma_kernel<128, BN, TB, 32, true><<<grid, kBlock, 0, st>>>(m, n, k, a, lda, b, ldb, part, n, 0, a_vec, b_vec, tiles_m, \
+    gemm_mfma_kernel<128, BN, TB, 32, true><<<grid, kBlock, 0, st>>>(m, n, k, a, lda, b, ldb, part, n, 0, tiles_m, \
                                                                      tiles_n, nullptr, 0, 1.0f, od, kNoInMask, kNoEpi, k_cut)
     if (trans_b)
         GCN_CUTS_GO(true);

@@ -251,25 +251,38 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_grad_kernel(NormGradArgs a, in
     }
 }
 
-// out[c] = sum over the rows of part [rows x f], 64 columns a workgroup, 16 strided sums a column added in order
+// out[c] = sum over the rows of part [rows x f]: 16 columns a workgroup, 64 strided sums a column, eight of their rows in
+// flight, added pairwise in a fixed tree.  (64 columns a workgroup and one row in flight: 38 us for 1974 x 256, 50 us for
+// 1924 x 1433; this form: 7 and 9 us.)
 __global__ __launch_bounds__(1024) void column_sums_kernel(int64_t rows, int f, const float* __restrict__ part,
                                                            float* __restrict__ out) {
-    __shared__ float lds[16][64];
-    const int col = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + col;
+    constexpr int kSlices = 64, kDepth = 8;
+    __shared__ float lds[kSlices][16];
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + col;
     float s = 0.0f;
-    if (c < f)
-        for (int64_t r = slice; r < rows; r += 16) s += part[r * f + c];
-    lds[slice][col] = s;
-    __syncthreads();
-    if (slice == 0 && c < f) {
-        for (int k = 1; k < 16; ++k) s += lds[k][col];
-        out[c] = s;
+    if (c < f) {
+        int64_t r = slice;
+        for (; r + (kDepth - 1) * kSlices < rows; r += kDepth * kSlices) {
+            float v[kDepth];
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) v[u] = part[(r + u * kSlices) * f + c];
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) s += v[u];
+        }
+        for (; r < rows; r += kSlices) s += part[r * f + c];
     }
+    lds[slice][col] = s;
+#pragma unroll
+    for (int half = kSlices / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (slice < half) lds[slice][col] += lds[slice + half][col];
+    }
+    if (slice == 0 && c < f) out[c] = lds[0][col];
 }
 
 int launch_column_sums(int64_t rows, int64_t f, const float* part, float* out, hipStream_t st) {
-    column_sums_kernel<<<(unsigned)ceil_div(f, (int64_t)64), 1024, 0, st>>>(rows, (int)f, part, out);
+    column_sums_kernel<<<(unsigned)ceil_div(f, (int64_t)16), 1024, 0, st>>>(rows, (int)f, part, out);
     GCN_LAUNCH_CHECK();
     return GCN_OK;
 }

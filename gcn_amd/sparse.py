@@ -5,6 +5,7 @@ into ``libgcn_hip.so`` through ``gcn_amd._lib``.
 """
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -930,23 +931,41 @@ def gather_rows(src, rows, out):
 _NO_GUARD = contextlib.nullcontext()
 
 
+# The helpers below are what a small call costs: on a citation graph a kernel takes 4 us and the call around it must
+# not take five times that.
 def _on_device(first, *others):
     """Context in which the device of ``first`` is the current one, so that a call enqueues on that device's current
     stream; the other tensors must live there too."""
-    _require_cuda(first, *others)
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError('gcn_amd operators take tensors that live on the GPU')
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError('the tensors of one call must live on one GPU: %s and %s' % (first.device, t.device))
-    return _NO_GUARD if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+    return _NO_GUARD if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _raw_stream():
+    """The current stream of the current device as the library takes it."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _matrix(x):
+    """``_rowmajor`` with a short way for what needs no change."""
+    return x if x.dtype is torch.float32 and x.dim() == 2 and x.is_contiguous() else _rowmajor(x)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _vector(x, n, what):
     """A contiguous float32 vector of n elements (or None)."""
     if x is None:
         return None
-    if x.dim() != 1 or x.numel() != n:
+    if x.dim() != 1 or x.shape[0] != n:
         raise ValueError('%s must be a vector of %d elements' % (what, n))
-    return x.float().contiguous()
+    return x if x.dtype is torch.float32 and x.is_contiguous() else x.float().contiguous()
 
 
 class QuantRows(object):
@@ -971,6 +990,7 @@ class QuantRows(object):
         return self.data.stride(0) if self.n_rows > 1 else (self.f + 15) // 16 * 16
 
     @staticmethod
+    @functools.lru_cache(maxsize=64)
     def pitch(f):
         out = ctypes.c_int64()
         _lib.call('gcn_quant_pitch', int(f), ctypes.byref(out))
@@ -978,9 +998,12 @@ class QuantRows(object):
 
     @classmethod
     def empty(cls, n_rows, f, device):
-        # torch's allocator returns 512-byte aligned blocks
-        return cls(n_rows, f, torch.empty((n_rows, cls.pitch(f)), dtype=torch.uint8, device=device),
-                   torch.empty(n_rows, dtype=torch.float32, device=device))
+        # torch's allocator returns 512-byte aligned blocks: what __init__ checks holds
+        rows = cls.__new__(cls)
+        rows.n_rows, rows.f = n_rows, f
+        rows.data = torch.empty((n_rows, cls.pitch(f)), dtype=torch.uint8, device=device)
+        rows.scales = torch.empty(n_rows, dtype=torch.float32, device=device)
+        return rows
 
     def rows(self, begin, end):
         """Rows begin .. end - 1 as QuantRows over the same memory."""
@@ -993,38 +1016,41 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=False, out=None, sum
     ``out``: where ``y`` goes (a float32 view, or QuantRows); ``sum_out``: where ``h`` goes, which may be ``x`` or
     ``residual`` itself.  A row holds at most 32768 columns.  ``h`` and ``inv`` are what ``rms_norm_grad`` wants."""
     with _on_device(x, weight, residual, sum_out):
-        x = _rowmajor(x)
+        x = _matrix(x)
         n, f = x.shape
         weight = _vector(weight, f, 'the weight')
         h = x
         if residual is not None:
-            residual = _rowmajor(residual)
+            residual = _matrix(residual)
             if residual.shape != x.shape:
                 raise ValueError('the residual has another shape than x')
             if sum_out is None:
-                h = torch.empty((n, f), dtype=torch.float32, device=x.device)
+                h = x.new_empty((n, f))
             else:
                 _check_out(sum_out, n, f)
                 h = sum_out
         elif sum_out is not None:
             raise ValueError('sum_out without a residual: h is x itself')
-        inv = torch.empty(n, dtype=torch.float32, device=x.device)
+        inv = x.new_empty(n)
         if quant:
-            y = QuantRows.empty(n, f, x.device) if out is None else out
-            if not isinstance(y, QuantRows) or y.n_rows != n or y.f != f or y.data.device != x.device:
+            if out is None:
+                y = QuantRows.empty(n, f, x.device)
+            elif isinstance(out, QuantRows) and out.n_rows == n and out.f == f and out.data.device == x.device:
+                y = out
+            else:
                 raise ValueError('out must be QuantRows of the shape of x')
-            args = (None, f, _p(y.data), y.ld, _p(y.scales))
+            args = (None, f, _at(y.data), y.ld, _at(y.scales))
         else:
             if out is None:
-                y = torch.empty((n, f), dtype=torch.float32, device=x.device)
+                y = x.new_empty((n, f))
             else:
                 _check_out(out, n, f)
                 y = out
                 if y.device != x.device:
                     raise ValueError('out lives on another GPU')
-            args = (_p(y), _ld(y), None, 0, None)
-        _lib.call('gcn_rms_norm_f32', n, f, _p(x), _ld(x), _p(residual), 0 if residual is None else _ld(residual),
-                  _p(weight), float(eps), _p(h) if residual is not None else None, _ld(h), _p(inv), *args, _stream())
+            args = (_at(y), _ld(y), None, 0, None)
+        _lib.call('gcn_rms_norm_f32', n, f, _at(x), _ld(x), _at(residual), 0 if residual is None else _ld(residual),
+                  _at(weight), float(eps), _at(h) if residual is not None else None, _ld(h), _at(inv), *args, _raw_stream())
     return y, h, inv
 
 
@@ -1034,21 +1060,21 @@ def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
     elsewhere.  ``dx`` is the gradient of x and of the residual alike.  ``dweight`` is summed over the rows in a fixed
     order (None without ``want_weight``)."""
     with _on_device(grad, h, weight, inv, grad_h):
-        grad, h = _rowmajor(grad), _rowmajor(h)
+        grad, h = _matrix(grad), _matrix(h)
         n, f = h.shape
         if grad.shape != h.shape or (grad_h is not None and grad_h.shape != h.shape):
             raise ValueError('shape mismatch in rms_norm_grad')
         weight, inv = _vector(weight, f, 'the weight'), _vector(inv, n, 'inv')
         if grad_h is not None:
-            grad_h = _rowmajor(grad_h)
-        dx = torch.empty((n, f), dtype=torch.float32, device=h.device)
+            grad_h = _matrix(grad_h)
+        dx = h.new_empty((n, f))
         dweight, ws, need = None, None, ctypes.c_size_t()
         if want_weight:
-            dweight = torch.empty(f, dtype=torch.float32, device=h.device)
+            dweight = h.new_empty(f)
             _lib.call('gcn_rms_norm_grad_workspace_bytes', n, f, ctypes.byref(need))
             ws = _workspace(need.value, h.device)
-        _lib.call('gcn_rms_norm_grad_f32', n, f, _p(grad), _ld(grad), _p(h), _ld(h), _p(weight), _p(inv), _p(grad_h),
-                  0 if grad_h is None else _ld(grad_h), _p(dx), f, _p(dweight), _p(ws), need.value, _stream())
+        _lib.call('gcn_rms_norm_grad_f32', n, f, _at(grad), _ld(grad), _at(h), _ld(h), _at(weight), _at(inv), _at(grad_h),
+                  0 if grad_h is None else _ld(grad_h), _at(dx), f, _at(dweight), _at(ws), need.value, _raw_stream())
     return dx, dweight
 
 
@@ -1063,15 +1089,15 @@ def spmm_quant(a, q, relu=False, out=None):
             raise ValueError('shape mismatch: %s @ 8-bit [%d x %d]' % (a.shape, q.n_rows, q.f))
         f = q.f
         if out is None:
-            out = torch.empty((a.n_rows, f), dtype=torch.float32, device=q.data.device)
+            out = q.scales.new_empty((a.n_rows, f))
         else:
             _check_out(out, a.n_rows, f)
         need, ws = ctypes.c_size_t(), None
         _lib.call('gcn_spmm_plan_workspace_bytes', a.plan.handle, f, ctypes.byref(need))
         if need.value:
             ws = _workspace(need.value, q.data.device)
-        _lib.call('gcn_spmm_csr_quant_f32', a.plan.handle, _p(a.indptr), _p(a.indices), _p(a.values), f, _p(q.data), q.ld,
-                  _p(q.scales), _p(out), _ld(out), _lib.GCN_RELU if relu else 0, _p(ws), need.value, _stream())
+        _lib.call('gcn_spmm_csr_quant_f32', a.plan.handle, _at(a.indptr), _at(a.indices), _at(a.values), f, _at(q.data), q.ld,
+                  _at(q.scales), _at(out), _ld(out), _lib.GCN_RELU if relu else 0, _at(ws), need.value, _raw_stream())
     return out
 
 
@@ -1094,29 +1120,29 @@ def gemm_epilogue(a, b, trans_b=False, bias=None, act=None, residual=None, out=N
     ``(result, pre)``, ``pre = a @ b + bias`` as ``act_grad`` wants it."""
     code = _act_code(act)
     with _on_device(a, b, bias, residual, out):
-        a, b = _rowmajor(a), _rowmajor(b)
+        a, b = _matrix(a), _matrix(b)
         m, k = a.shape
         n = b.shape[0] if trans_b else b.shape[1]
         if (b.shape[1] if trans_b else b.shape[0]) != k:
             raise ValueError('shape mismatch in gemm_epilogue')
         bias = _vector(bias, n, 'the bias')
         if residual is not None:
-            residual = _rowmajor(residual)
+            residual = _matrix(residual)
             if tuple(residual.shape) != (m, n):
                 raise ValueError('the residual must have the shape of the result')
         if out is None:
-            c = torch.empty((m, n), dtype=torch.float32, device=a.device)
+            c = a.new_empty((m, n))
         else:
             _check_out(out, m, n)
             c = out
-        pre = torch.empty((m, n), dtype=torch.float32, device=a.device) if want_pre else None
+        pre = a.new_empty((m, n)) if want_pre else None
         need, ws = ctypes.c_size_t(), None
         _lib.call('gcn_gemm_epilogue_workspace_bytes', m, n, k, ctypes.byref(need))
         if need.value:
             ws = _workspace(need.value, a.device)
-        _lib.call('gcn_gemm_epilogue_f32', m, n, k, _p(a), _ld(a), _p(b), _ld(b), 1 if trans_b else 0, _p(bias), code,
-                  _p(residual), 0 if residual is None else _ld(residual), _p(pre), n, _p(c), _ld(c), _p(ws), need.value,
-                  _stream())
+        _lib.call('gcn_gemm_epilogue_f32', m, n, k, _at(a), _ld(a), _at(b), _ld(b), 1 if trans_b else 0, _at(bias), code,
+                  _at(residual), 0 if residual is None else _ld(residual), _at(pre), n, _at(c), _ld(c), _at(ws), need.value,
+                  _raw_stream())
     return (c, pre) if want_pre else c
 
 
@@ -1126,24 +1152,24 @@ def act_grad(grad, pre, act, want_bias=True):
     ``gemm_tn(a, dz)`` and, for the residual, ``grad``."""
     code = _act_code(act)
     with _on_device(grad, pre):
-        grad = _rowmajor(grad)
+        grad = _matrix(grad)
         m, n = grad.shape
         if code != _lib.GCN_ACT_NONE:
             if pre is None:
                 raise ValueError('the gradient of an activation wants the pre-activation')
-            pre = _rowmajor(pre)
+            pre = _matrix(pre)
             if pre.shape != grad.shape:
                 raise ValueError('the pre-activation has another shape than the gradient')
-            dz = torch.empty((m, n), dtype=torch.float32, device=grad.device)
+            dz = grad.new_empty((m, n))
         else:
             pre, dz = None, None
         dbias, ws, need = None, None, ctypes.c_size_t()
         if want_bias:
-            dbias = torch.empty(n, dtype=torch.float32, device=grad.device)
+            dbias = grad.new_empty(n)
             _lib.call('gcn_act_grad_workspace_bytes', m, n, ctypes.byref(need))
             ws = _workspace(need.value, grad.device)
-        _lib.call('gcn_act_grad_f32', m, n, code, _p(grad), _ld(grad), _p(pre), 0 if pre is None else _ld(pre), _p(dz), n,
-                  _p(dbias), _p(ws), need.value, _stream())
+        _lib.call('gcn_act_grad_f32', m, n, code, _at(grad), _ld(grad), _at(pre), 0 if pre is None else _ld(pre), _at(dz), n,
+                  _at(dbias), _at(ws), need.value, _raw_stream())
     return (grad if dz is None else dz), dbias
 
 
@@ -1162,7 +1188,7 @@ def distill_topk(logits, values, indices, mask, mask_mean, temperature=1.0, want
     ``loss_summary`` averages; ``grad``: the gradient of their mean w.r.t. the logits, times ``upstream`` (a float32
     device scalar) if given."""
     with _on_device(logits, values, indices, mask, upstream):
-        logits = _rowmajor(logits)
+        logits = _matrix(logits)
         n, c = logits.shape
         if values.dtype not in _VALUE_TYPES:
             raise ValueError("the teacher's logits must be float32, float16 or bfloat16")
@@ -1176,9 +1202,9 @@ def distill_topk(logits, values, indices, mask, mask_mean, temperature=1.0, want
         values, indices = values.contiguous(), indices.contiguous()
         mask = None if mask is None else mask.contiguous()
         k = values.shape[1]
-        stats = torch.empty((n, 2), dtype=torch.float32, device=logits.device) if want_stats else None
-        grad = torch.empty((n, c), dtype=torch.float32, device=logits.device) if want_grad else None
-        _lib.call('gcn_distill_topk_f32', n, c, _p(logits), _ld(logits), _p(values), _VALUE_TYPES[values.dtype], k,
-                  _p(indices), k, k, _p(mask), float(mask_mean), float(temperature), _p(upstream), _p(stats), _p(grad), c,
-                  _stream())
+        stats = logits.new_empty((n, 2)) if want_stats else None
+        grad = logits.new_empty((n, c)) if want_grad else None
+        _lib.call('gcn_distill_topk_f32', n, c, _at(logits), _ld(logits), _at(values), _VALUE_TYPES[values.dtype], k,
+                  _at(indices), k, k, _at(mask), float(mask_mean), float(temperature), _at(upstream), _at(stats), _at(grad), c,
+                  _raw_stream())
     return stats, grad
