@@ -6,10 +6,12 @@
 //   agreement = w where argmax s (ties: the lowest class) is the class of the largest listed logit (ties: the first listed)
 //
 // Bound by memory: the logits are read once and their gradient is written once, the exponentials of a row staying in
-// registers between the two; rows outside the mask are not read at all.  Rows of up to 256 classes belong to G lanes
-// with four consecutive classes each, so that a wave holds 64 / G rows and the eight reductions a row needs are shared
-// by them; wider ones to a wave or a workgroup, up to 65,536 classes; beyond that the row is read a second time for
-// its gradient.
+// registers between the two; rows outside the mask are not read at all.  Rows of up to 256 classes belong to G lanes with
+// four or eight classes each, so that a wave holds 64 / G rows and the reductions a row needs are shared by them; wider
+// ones to a wave or a workgroup, up to 65,536 classes; beyond that the row is read a second time for its gradient.
+// Measured, compulsory bytes over time (a large copy: 4.7 TB/s): 4 M x 47 classes, 5 listed: 390 us, 4.5 TB/s;
+// 4 M x 7, 3 listed: 90 us, 4.0; 1 M x 200, 20 listed: 389 us, 4.7; 8,192 x 32,768, 32 listed: 416 us, 5.2;
+// 2,048 x 65,536: 426 us, 2.5 (one workgroup a compute unit, and it spills).
 #include <algorithm>
 #include <hip/hip_fp16.h>
 
@@ -34,131 +36,261 @@ struct DistillArgs {
     int64_t ldi;
     int k;
     const int32_t* mask;      // may be null: all ones
-    float inv_mask_mean, inv_t, t;
+    float inv_mask_mean, t, to_log2;      // t: the temperature; to_log2: log2(e) / t
     float* stats;             // [n x 2] or null
     float* grad;              // [n x c] or null
     int64_t ldg;
     const float* upstream;    // device scalar the gradient is multiplied by, or null
 };
 
-__device__ __forceinline__ float teacher_value(const DistillArgs& a, int64_t row, int j) {
-    const int64_t at = row * a.ldv + j;
-    if (a.type == GCN_F32) return static_cast<const float*>(a.values)[at];
-    if (a.type == GCN_F16) return __half2float(static_cast<const __half*>(a.values)[at]);
-    return __uint_as_float((uint32_t) static_cast<const uint16_t*>(a.values)[at] << 16);
-}
-
-// One entry of the teacher's list: its logit over the temperature, -inf where it is no entry.
+// One entry of the teacher's list: its logit, -inf and no class where it is no entry.
 struct Entry {
     float t;
     int at;
 };
-__device__ __forceinline__ Entry teacher_entry(const DistillArgs& a, int64_t row, int j) {
-    Entry e = {-INFINITY, -1};
+// The same as loaded: the 32-bit word that holds the logit (of a 16-bit logit the whole aligned word, inside the
+// allocation whatever its address), where in it, and the class.  Nothing here depends on a loaded value and nothing branches
+// on the type, so that a list can be fetched ahead of its use.
+struct RawEntry {
+    uint32_t word;
+    int shift, at;
+};
+__device__ __forceinline__ RawEntry fetch_entry(const DistillArgs& a, int64_t row, int j) {
+    RawEntry r = {0u, 0, -1};
     if (j < a.k) {
-        const int at = a.indices[row * a.ldi + j];
-        if (at >= 0 && at < a.c) {
-            e.t = teacher_value(a, row, j) * a.inv_t;
-            e.at = at;
+        const uintptr_t where = (uintptr_t)a.values + ((uint64_t)(row * a.ldv + j) << (a.type == GCN_F32 ? 2 : 1));
+        r.word = *reinterpret_cast<const uint32_t*>(where & ~(uintptr_t)3);
+        r.shift = (int)(where & 2) * 8;
+        r.at = a.indices[row * a.ldi + j];
+    }
+    return r;
+}
+__device__ __forceinline__ Entry entry_of(const DistillArgs& a, const RawEntry& r) {
+    const uint32_t half = (r.word >> r.shift) & 0xffffu;
+    const float f16 = __half2float(__builtin_bit_cast(__half, (uint16_t)half));
+    const float t = a.type == GCN_F32 ? __uint_as_float(r.word) : a.type == GCN_F16 ? f16 : __uint_as_float(half << 16);
+    const bool in = r.at >= 0 && r.at < a.c;
+    return {in ? t : -INFINITY, in ? r.at : -1};
+}
+__device__ __forceinline__ Entry teacher_entry(const DistillArgs& a, int64_t row, int j) {
+    return entry_of(a, fetch_entry(a, row, j));
+}
+
+// LDS accesses of one wave stay in program order; this keeps the compiler to it.
+__device__ __forceinline__ void lds_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Exponents and logarithms are base 2 (one instruction each): a logit's exponent is (s - max) log2(e) / T.
+// The loss row from its parts: tsum = sum 2^d_j, tdot = sum 2^d_j d_j (d_j: the exponents of the list), qdot = sum p_j log2 q_j.
+__device__ __forceinline__ float row_loss(const DistillArgs& a, float tsum, float tdot, float qdot, float w) {
+    const float kLn2 = 0.6931471805599453f;
+    return (tdot * __builtin_amdgcn_rcpf(tsum) - __builtin_amdgcn_logf(tsum) - qdot) * (kLn2 * a.t * a.t * w);
+}
+
+// ------------------------------------------------------------------------------------------------
+// c <= 4 G VPL: G lanes a row, 64 / G rows a wave
+// ------------------------------------------------------------------------------------------------
+// The rows of a group are a pipeline: the mask is fetched two rows ahead and the logits and the list one row ahead of the
+// row in work, nothing of the fetch depending on a loaded value.  A row outside the
+// mask is a row without entries whose logits are not loaded: it takes the same way and ends as zeros.
+// P, the teacher's probabilities by class, is made in LDS: every entry writes its number at its class and reads it back;
+// if all find their own, no class is listed twice and they write their exponentials there.  Otherwise the wave adds the
+// entries one by one in list order.
+template <int G, int VPL>
+__device__ __forceinline__ void load_logits(const float* __restrict__ row, int sub, int c, bool last, float (&x)[VPL][4]) {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        // a vector that begins in the row may end in the next one, whose values are replaced below; behind the last
+        // row there may be nothing
+        const int at = 4 * (sub + G * v);
+        if (!last || at + 4 <= c) {
+            const f4u f = *reinterpret_cast<const f4u*>(row + (at < c ? at : 0));
+            x[v][0] = f.x;
+            x[v][1] = f.y;
+            x[v][2] = f.z;
+            x[v][3] = f.w;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[v][q] = at + q < c ? row[at + q] : 0.0f;
         }
     }
-    return e;
+}
+// the row's columns; the one vector that the row's end cuts is stored by one instruction of its length
+template <int G, int VPL>
+__device__ __forceinline__ void store_grad(float* __restrict__ row, int sub, int c, const float (&g)[VPL][4]) {
+    const int cut = c & 3;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+        const int at = 4 * (sub + G * v);
+        if (at + 4 <= c) *reinterpret_cast<f4u*>(row + at) = f4u{g[v][0], g[v][1], g[v][2], g[v][3]};
+        if (cut != 0 && at < c && at + 4 > c) {
+            typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+            typedef float f3u __attribute__((ext_vector_type(3), aligned(4)));
+            if (cut == 1) row[at] = g[v][0];
+            else if (cut == 2) *reinterpret_cast<f2u*>(row + at) = f2u{g[v][0], g[v][1]};
+            else *reinterpret_cast<f3u*>(row + at) = f3u{g[v][0], g[v][1], g[v][2]};
+        }
+    }
 }
 
-// the loss row from its parts: tsum = sum e_j, tdot = sum e_j (t_j - tmax), qdot = sum p_j log q_j.  Without an entry: 0.
-__device__ __forceinline__ float row_loss(float tsum, float tdot, float qdot, float t2w) {
-    return (tdot / tsum - logf(tsum) - qdot) * t2w;
-}
-
-// ------------------------------------------------------------------------------------------------
-// c <= 4 G: G lanes a row
-// ------------------------------------------------------------------------------------------------
-template <int G>
+// A lane holds NE entries of the list in registers (G NE of them a row); MORE: longer lists, whose other entries are read
+// again by every pass over the list (17 entries on 47 classes: 1.13 ms against 0.48 in registers).
+template <int G, int VPL, int NE, bool MORE>
 __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int tile) {
     constexpr int kRows = 256 / G;
-    const int sub = threadIdx.x % G, c0 = 4 * sub;
+    __shared__ __attribute__((aligned(16))) float by_class[kRows][4 * G * VPL];
+    const int sub = threadIdx.x % G, group = threadIdx.x / G;
+    float* const mine = by_class[group];
     const float up = (a.upstream ? *a.upstream : 1.0f) * a.t * a.per_row;
-    const int64_t base = (int64_t)blockIdx.x * tile * kRows;
-    for (int t = 0; t < tile; ++t) {
-        const int64_t i = base + (int64_t)t * kRows + threadIdx.x / G;
-        if (base + (int64_t)t * kRows >= a.n) break;
-        const bool live = i < a.n;
-        const int m = live ? (a.mask ? a.mask[i] : 1) : 0;
-        const float w = (float)m * a.inv_mask_mean;
-        if (live && m == 0) {
-            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (a.grad && c0 < a.c) store_cols(a.grad + i * a.ldg, c0, a.c, zero);
-            if (a.stats && sub == 0) *reinterpret_cast<float2*>(a.stats + 2 * i) = make_float2(0.0f, 0.0f);
+    const int64_t base = (int64_t)blockIdx.x * tile * kRows + group;
+    const int rows = (int)(base >= a.n ? 0 : std::min<int64_t>(tile, (a.n - base + kRows - 1) / kRows));   // of this group
+    const int left = a.c - 4 * sub;                  // columns from the lane's first one on
+    auto load_mask = [&](int t) { return t < rows ? (a.mask ? a.mask[base + (int64_t)t * kRows] : 1) : 0; };
+    auto load_row = [&](int t, int m, float (&x)[VPL][4], RawEntry (&e)[NE]) {
+#pragma unroll
+        for (int u = 0; u < NE; ++u) e[u] = {0u, 0, -1};
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[v][q] = 0.0f;
+        if (m != 0) {
+            const int64_t i = base + (int64_t)t * kRows;
+            load_logits<G, VPL>(a.logits + i * a.ldx, sub, a.c, i == a.n - 1, x);
+#pragma unroll
+            for (int u = 0; u < NE; ++u) e[u] = fetch_entry(a, i, G * u + sub);
         }
-        if (m == 0) continue;                            // the lanes of a row agree; reductions stay inside the row
-        float x[4], p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        load_cols(a.logits + i * a.ldx, c0 < a.c ? c0 : 0, a.c, x);
-        // the teacher's entries, G at a time; lists of at most G entries are read once
-        Entry e = teacher_entry(a, i, sub);
-        float tmax = e.t;
-        for (int j = G; j < a.k; j += G) tmax = fmaxf(tmax, teacher_entry(a, i, j + sub).t);
+    };
+    float nx[VPL][4];
+    RawEntry ne[NE];
+    int nm = load_mask(0);
+    load_row(0, nm, nx, ne);
+    int nnm = load_mask(1);
+    for (int t = 0; t < tile; ++t) {
+        if ((int64_t)blockIdx.x * tile * kRows + (int64_t)t * kRows >= a.n) break;      // uniform in the workgroup
+        const int64_t i = base + (int64_t)t * kRows;
+        const bool live = t < rows;
+        const int m = nm;
+        Entry e0[NE];
+#pragma unroll
+        for (int u = 0; u < NE; ++u) e0[u] = entry_of(a, ne[u]);
+        // calls f(entry, its number) for the lane's entries, in list order
+        auto entries = [&](auto f) {
+#pragma unroll
+            for (int u = 0; u < NE; ++u) f(e0[u], G * u + sub);
+            if (MORE)
+                for (int j = G * NE; j < a.k; j += G) f(m != 0 ? teacher_entry(a, i, j + sub) : Entry{-INFINITY, -1}, j + sub);
+        };
+        float x[VPL][4], xm = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                x[v][q] = 4 * G * v + q < left ? nx[v][q] : -INFINITY;
+                xm = fmaxf(xm, x[v][q]);
+            }
+        nm = nnm;
+        load_row(t + 1, nm, nx, ne);
+        nnm = load_mask(t + 2);
+        const float w = (float)m * a.inv_mask_mean;
+        xm = lanes_reduce<G, OpMax>(xm);
+        float tmax = -INFINITY;
+        entries([&](const Entry& e, int) { tmax = fmaxf(tmax, e.t); });
         tmax = lanes_reduce<G, OpMax>(tmax);
         const float tref = tmax > -INFINITY ? tmax : 0.0f;
-        float xm = -INFINITY;
+        // the list: its sums, its first maximum, P
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (c0 + q < a.c) xm = fmaxf(xm, x[q]);
-        xm = lanes_reduce<G, OpMax>(xm);
-        int first = 0x7fffffff;
-#pragma unroll
-        for (int q = 3; q >= 0; --q)
-            if (c0 + q < a.c && x[q] == xm) first = c0 + q;
-        float s = 0.0f, z[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            z[q] = (x[q] - xm) * a.inv_t;
-            x[q] = c0 + q < a.c ? expf(z[q]) : 0.0f;
-            s += x[q];
-        }
-        s = lanes_reduce<G, OpAdd>(s);
+        for (int v = 0; v < VPL; ++v)
+            *reinterpret_cast<float4*>(mine + 4 * (sub + G * v)) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        lds_in_order();
+        entries([&](const Entry& e, int number) {
+            if (e.at >= 0) mine[e.at] = __int_as_float(number + 1);
+        });
+        lds_in_order();
         float tsum = 0.0f, tdot = 0.0f;
-        int top = 0x7fffffff;
-        for (int j = 0; j < a.k; j += G) {
-            if (j > 0) e = teacher_entry(a, i, j + sub);
-            const float d = e.t - tref, ex = e.at >= 0 ? expf(d) : 0.0f;
+        int top = 0x7fffffff, top_at = -1;
+        bool twice = false;
+        entries([&](const Entry& e, int number) {
+            const int found = __float_as_int(mine[max(e.at, 0)]);
+            twice = twice || (e.at >= 0 && found != number + 1);
+            const float d = (e.t - tref) * a.to_log2, ex = e.at >= 0 ? __builtin_amdgcn_exp2f(d) : 0.0f;
             tsum += ex;
-            if (ex > 0.0f) tdot = fmaf(ex, d, tdot);
-            if (e.at >= 0 && e.t == tmax) top = min(top, j + sub);
-            const int here = min(G, a.k - j);
-            for (int b = 0; b < here; ++b) {
-                const float exb = __shfl(ex, b, G);
-                const int at = __shfl(e.at, b, G) - c0;
+            tdot = fmaf(ex, ex > 0.0f ? d : 0.0f, tdot);
+            const bool here = e.at >= 0 && e.t == tmax && top_at < 0;
+            top = here ? number : top;
+            top_at = here ? e.at : top_at;
+        });
+        lds_in_order();
+        float p[VPL][4];
+        if (__any(twice)) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) p[q] += at == q ? exb : 0.0f;
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) p[v][q] = 0.0f;
+            entries([&](const Entry& e, int number) {
+                const float ex = e.at >= 0 ? __builtin_amdgcn_exp2f((e.t - tref) * a.to_log2) : 0.0f;
+                const int here = min(G, a.k - (number - sub));           // the entries the row's lanes hold now
+                for (int b = 0; b < here; ++b) {
+                    const float exb = __shfl(ex, b, G);
+                    const int at = __shfl(e.at, b, G) - 4 * sub;
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) p[v][q] += at == 4 * G * v + q ? exb : 0.0f;
+                }
+            });
+        } else {
+            entries([&](const Entry& e, int) {
+                if (e.at >= 0) mine[e.at] = __builtin_amdgcn_exp2f((e.t - tref) * a.to_log2);
+            });
+            lds_in_order();
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                const float4 f = *reinterpret_cast<const float4*>(mine + 4 * (sub + G * v));
+                p[v][0] = f.x;
+                p[v][1] = f.y;
+                p[v][2] = f.z;
+                p[v][3] = f.w;
             }
         }
+        lds_in_order();
         tsum = lanes_reduce<G, OpAdd>(tsum);
         const bool any = tmax > -INFINITY || !(tsum == 0.0f);       // a NaN logit of the teacher is an entry
-        const float pscale = any ? 1.0f / tsum : 0.0f;
-        const float logs = logf(s);
-        float qdot = 0.0f;
+        const float pscale = any ? __builtin_amdgcn_rcpf(tsum) : 0.0f;
+        // the student; columns past the end are -inf and add nothing
+        int first = 0x7fffffff;
+        float s = 0.0f, dot = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            p[q] *= pscale;
-            if (!(p[q] == 0.0f)) qdot = fmaf(p[q], z[q] - logs, qdot);
-        }
+        for (int v = VPL - 1; v >= 0; --v)
+#pragma unroll
+            for (int q = 3; q >= 0; --q) {
+                first = x[v][q] == xm ? 4 * (sub + G * v) + q : first;
+                const float z = (x[v][q] - xm) * a.to_log2;
+                x[v][q] = __builtin_amdgcn_exp2f(z);
+                s += x[v][q];
+                p[v][q] *= pscale;
+                dot = fmaf(p[v][q], p[v][q] == 0.0f ? 0.0f : z, dot);
+            }
+        s = lanes_reduce<G, OpAdd>(s);
         if (a.stats) {
             tdot = lanes_reduce<G, OpAdd>(tdot);
-            qdot = lanes_reduce<G, OpAdd>(qdot);
+            dot = lanes_reduce<G, OpAdd>(dot);
             first = __float_as_int(lanes_reduce<G, OpMinInt>(__int_as_float(first)));
-            top = __float_as_int(lanes_reduce<G, OpMinInt>(__int_as_float(top)));
-            if (sub == 0) {
-                const int best = top < a.k ? a.indices[i * a.ldi + top] : -1;
-                *reinterpret_cast<float2*>(a.stats + 2 * i) =
-                    make_float2(any ? row_loss(tsum, tdot, qdot, w * a.t * a.t) : 0.0f, any && first == best ? w : 0.0f);
-            }
+            const int best = __float_as_int(lanes_reduce<G, OpMinInt>(__int_as_float(top)));
+            // sum p log q = sum p z - log2(s): the p add up to 1
+            const float hit = lanes_reduce<G, OpMax>(top_at >= 0 && top == best && top_at == first ? w : 0.0f);
+            const float loss = row_loss(a, tsum, tdot, dot - __builtin_amdgcn_logf(s), w);
+            if (live && sub == 0)
+                *reinterpret_cast<float2*>(a.stats + 2 * i) = make_float2(any ? loss : 0.0f, any ? hit : 0.0f);
         }
-        if (a.grad && c0 < a.c) {
-            const float scale = w * up, qs = 1.0f / s;
-            float g[4];
+        if (a.grad) {
+            const float scale = w * up, qs = __builtin_amdgcn_rcpf(s);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) g[q] = any ? (x[q] * qs - p[q]) * scale : 0.0f;
-            store_cols(a.grad + i * a.ldg, c0, a.c, g);
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[v][q] = any ? (x[v][q] * qs - p[v][q]) * scale : 0.0f;
+            if (live) store_grad<G, VPL>(a.grad + i * a.ldg, sub, a.c, x);
         }
     }
 }
@@ -198,7 +330,7 @@ __device__ __forceinline__ Listed list_entries(const DistillArgs& a, int64_t i, 
     Listed l = {0.0f, 0.0f, 0x7fffffff, false};
 #pragma unroll
     for (int b = 0; b < kDistillMaxK / 64; ++b) {
-        const float d = e[b].t - tref, ex = e[b].at >= 0 ? expf(d) : 0.0f;
+        const float d = (e[b].t - tref) * a.to_log2, ex = e[b].at >= 0 ? __builtin_amdgcn_exp2f(d) : 0.0f;
         l.tsum += ex;
         if (ex > 0.0f) l.tdot = fmaf(ex, d, l.tdot);
         if (e[b].at >= 0 && e[b].t == tmax) l.top = min(l.top, 64 * b + lane);
@@ -208,8 +340,7 @@ __device__ __forceinline__ Listed list_entries(const DistillArgs& a, int64_t i, 
     l.tdot = lanes_reduce<64, OpAdd>(l.tdot);
     l.top = __float_as_int(lanes_reduce<64, OpMinInt>(__int_as_float(l.top)));
     l.any = tmax > -INFINITY || !(l.tsum == 0.0f);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the list is read by other lanes of this wave
-    __builtin_amdgcn_wave_barrier();
+    lds_in_order();                                              // the list is read by other lanes of this wave
     l.top = l.top < a.k ? __float_as_int(list[l.top].y) : -1;
     return l;
 }
@@ -238,7 +369,7 @@ __device__ __forceinline__ float listed_log_q(const DistillArgs& a, int64_t i, i
     for (int j = lane; j < a.k; j += 64) {
         const float2 v = list[j];
         if (__float_as_int(v.y) >= 0 && !(v.x == 0.0f))
-            qdot = fmaf(v.x * pscale, (a.logits[i * a.ldx + __float_as_int(v.y)] - xm) * a.inv_t - logs, qdot);
+            qdot = fmaf(v.x * pscale, (a.logits[i * a.ldx + __float_as_int(v.y)] - xm) * a.to_log2 - logs, qdot);
     }
     return lanes_reduce<64, OpAdd>(qdot);
 }
@@ -249,7 +380,7 @@ __device__ __forceinline__ void listed_grad(const DistillArgs& a, int64_t i, int
         const int at = __float_as_int(list[j].y);
         float sum;
         if (sum_of_class(list, a.k, j, at, &sum)) {
-            const float q = expf((a.logits[i * a.ldx + at] - xm) * a.inv_t) * qs;
+            const float q = __builtin_amdgcn_exp2f((a.logits[i * a.ldx + at] - xm) * a.to_log2) * qs;
             a.grad[i * a.ldg + at] = (q - sum * pscale) * scale;
         }
     }
@@ -280,22 +411,22 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
         return;
     }
     float x[VPL][4];
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        const int c = 4 * (sub + G * j);
-        load_cols(xr, c < a.c ? c : 0, a.c, x[j]);
-    }
+    load_logits<G, VPL>(xr, sub, a.c, i == a.n - 1, x);
     Listed l;
     if (lister) {
         l = list_entries(a, i, lane, list);
         if (G > 64 && lane == 0) shared_list[slot] = l;
     }
+    // columns past the end are -inf and add nothing
+    const int left = a.c - 4 * sub;
     float xm = -INFINITY;
 #pragma unroll
     for (int j = 0; j < VPL; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (4 * (sub + G * j) + q < a.c) xm = fmaxf(xm, x[j][q]);
+        for (int q = 0; q < 4; ++q) {
+            x[j][q] = 4 * G * j + q < left ? x[j][q] : -INFINITY;
+            xm = fmaxf(xm, x[j][q]);
+        }
     xm = wide_reduce<G, OpMax>(xm, lds[0]);
     if (G > 64) l = shared_list[slot];
     int first = 0x7fffffff;
@@ -304,9 +435,8 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     for (int j = VPL - 1; j >= 0; --j)
 #pragma unroll
         for (int q = 3; q >= 0; --q) {
-            const int c = 4 * (sub + G * j) + q;
-            if (c < a.c && x[j][q] == xm) first = c;
-            x[j][q] = c < a.c ? expf((x[j][q] - xm) * a.inv_t) : 0.0f;
+            first = x[j][q] == xm ? 4 * (sub + G * j) + q : first;
+            x[j][q] = __builtin_amdgcn_exp2f((x[j][q] - xm) * a.to_log2);
             s += x[j][q];
         }
     s = wide_reduce<G, OpAdd>(s, lds[1]);
@@ -317,21 +447,18 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     if (gr) {
         const float all = l.any ? qs * scale : 0.0f;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            const int c = 4 * (sub + G * j);
-            float g[4];
+        for (int j = 0; j < VPL; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) g[q] = l.any ? x[j][q] * all : 0.0f;
-            if (c < a.c) store_cols(gr, c, a.c, g);
-        }
+            for (int q = 0; q < 4; ++q) x[j][q] = l.any ? x[j][q] * all : 0.0f;
+        store_grad<G, VPL>(gr, sub, a.c, x);
     }
     if (a.stats) {
         first = __float_as_int(wide_reduce<G, OpMinInt>(__int_as_float(first), lds[2]));
         if (lister) {
-            const float qdot = listed_log_q(a, i, lane, list, xm, logf(s), pscale);
+            const float qdot = listed_log_q(a, i, lane, list, xm, __builtin_amdgcn_logf(s), pscale);
             if (lane == 0)
                 *reinterpret_cast<float2*>(a.stats + 2 * i) =
-                    make_float2(l.any ? row_loss(l.tsum, l.tdot, qdot, w * a.t * a.t) : 0.0f,
+                    make_float2(l.any ? row_loss(a, l.tsum, l.tdot, qdot, w) : 0.0f,
                                 l.any && first == l.top ? w : 0.0f);
         }
     }
@@ -372,30 +499,30 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     for (int64_t c = tid; c < a.c; c += G) {
         const float v = xr[c];
         if (v > run) {
-            s *= expf((run - v) * a.inv_t);
+            s *= __builtin_amdgcn_exp2f((run - v) * a.to_log2);
             run = v;
             first = (int)c;
         }
-        s += v == -INFINITY ? 0.0f : expf((v - run) * a.inv_t);
+        s += v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v - run) * a.to_log2);
     }
     const float xm = wide_reduce<G, OpMax>(run, lds[0]);
     const Listed l = shared_list;
     if (run != xm) first = 0x7fffffff;
-    s = run == -INFINITY && s == 0.0f ? (xm == -INFINITY ? NAN : 0.0f) : s * expf((run - xm) * a.inv_t);
+    s = run == -INFINITY && s == 0.0f ? (xm == -INFINITY ? NAN : 0.0f) : s * __builtin_amdgcn_exp2f((run - xm) * a.to_log2);
     s = wide_reduce<G, OpAdd>(s, lds[1]);
     const float pscale = l.any ? 1.0f / l.tsum : 0.0f;
     // a NaN among the listed logits makes the whole row NaN, as it does where P covers every class
     const float scale = l.tsum == l.tsum ? w * (a.upstream ? *a.upstream : 1.0f) * a.t * a.per_row : NAN;
     const float qs = 1.0f / s;
     if (gr)
-        for (int64_t c = tid; c < a.c; c += G) gr[c] = l.any ? expf((xr[c] - xm) * a.inv_t) * (qs * scale) : 0.0f;
+        for (int64_t c = tid; c < a.c; c += G) gr[c] = l.any ? __builtin_amdgcn_exp2f((xr[c] - xm) * a.to_log2) * (qs * scale) : 0.0f;
     if (a.stats) {
         first = __float_as_int(wide_reduce<G, OpMinInt>(__int_as_float(first), lds[2]));
         if (tid < 64) {
-            const float qdot = listed_log_q(a, i, lane, list, xm, logf(s), pscale);
+            const float qdot = listed_log_q(a, i, lane, list, xm, __builtin_amdgcn_logf(s), pscale);
             if (lane == 0)
                 *reinterpret_cast<float2*>(a.stats + 2 * i) =
-                    make_float2(l.any ? row_loss(l.tsum, l.tdot, qdot, w * a.t * a.t) : 0.0f,
+                    make_float2(l.any ? row_loss(a, l.tsum, l.tdot, qdot, w) : 0.0f,
                                 l.any && first == l.top ? w : 0.0f);
         }
     }
@@ -404,12 +531,20 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     if (tid < 64) listed_grad(a, i, lane, list, xm, qs, pscale, scale);
 }
 
-template <int G>
+template <int G, int VPL>
 static void launch_group(const DistillArgs& a, hipStream_t st) {
     constexpr int kRows = 256 / G;
     // one group of rows a workgroup until there are 16 workgroups for every compute unit
     const int tile = (int)std::min<int64_t>(8, std::max<int64_t>(1, ceil_div(a.n, (int64_t)kRows) / 4096));
-    distill_group_kernel<G><<<(unsigned)ceil_div(a.n, (int64_t)kRows * tile), 256, 0, st>>>(a, tile);
+    const unsigned blocks = (unsigned)ceil_div(a.n, (int64_t)kRows * tile);
+    if (a.k <= G)
+        distill_group_kernel<G, VPL, 1, false><<<blocks, 256, 0, st>>>(a, tile);
+    else if (a.k <= 2 * G)
+        distill_group_kernel<G, VPL, 2, false><<<blocks, 256, 0, st>>>(a, tile);
+    else if (a.k <= 4 * G)
+        distill_group_kernel<G, VPL, 4, false><<<blocks, 256, 0, st>>>(a, tile);
+    else
+        distill_group_kernel<G, VPL, 4, true><<<blocks, 256, 0, st>>>(a, tile);
 }
 
 template <int G, int VPL, int BLOCK>
@@ -417,14 +552,16 @@ static void launch_row(const DistillArgs& a, hipStream_t st) {
     distill_row_kernel<G, VPL, BLOCK><<<(unsigned)ceil_div(a.n, (int64_t)(BLOCK / G)), BLOCK, 0, st>>>(a);
 }
 
+// Lanes and vectors a row.  Two vectors a lane from 17 classes on: half the reductions a row (25 classes: 232 us against 261
+// with one; 47 classes: 390 against 478, and 412 with four); below, the longer pipelines of entries cost more than that.
 static void launch_distill(const DistillArgs& a, hipStream_t st) {
-    if (a.c <= 4) launch_group<1>(a, st);
-    else if (a.c <= 8) launch_group<2>(a, st);
-    else if (a.c <= 16) launch_group<4>(a, st);
-    else if (a.c <= 32) launch_group<8>(a, st);
-    else if (a.c <= 64) launch_group<16>(a, st);
-    else if (a.c <= 128) launch_group<32>(a, st);
-    else if (a.c <= 256) launch_group<64>(a, st);
+    if (a.c <= 4) launch_group<1, 1>(a, st);
+    else if (a.c <= 8) launch_group<2, 1>(a, st);
+    else if (a.c <= 16) launch_group<4, 1>(a, st);
+    else if (a.c <= 32) launch_group<4, 2>(a, st);
+    else if (a.c <= 64) launch_group<8, 2>(a, st);
+    else if (a.c <= 128) launch_group<16, 2>(a, st);
+    else if (a.c <= 256) launch_group<32, 2>(a, st);
     else if (a.c <= 512) launch_row<64, 2, 256>(a, st);
     else if (a.c <= 1024) launch_row<64, 4, 256>(a, st);
     else if (a.c <= 4096) launch_row<256, 4, 256>(a, st);
@@ -463,7 +600,7 @@ int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx,
     for (int64_t r = 0; r < n; r += kSlice) {
         const DistillArgs a = {std::min(kSlice, n - r), 1.0f / (float)n, (int)c, logits + r * ldx, ldx,
                                (const char*)values + r * ldv * value_size, value_type, ldv, indices + r * ldi, ldi, (int)k,
-                               mask ? mask + r : nullptr, 1.0f / mask_mean, 1.0f / temperature, temperature,
+                               mask ? mask + r : nullptr, 1.0f / mask_mean, temperature, 1.4426950408889634f / temperature,
                                row_stats ? row_stats + 2 * r : nullptr, dlogits ? dlogits + r * ldd : nullptr, ldd, upstream};
         launch_distill(a, (hipStream_t)stream);
         GCN_LAUNCH_CHECK();
