@@ -98,43 +98,6 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, float tsum, floa
 // P, the teacher's probabilities by class, is made in LDS: every entry writes its number at its class and reads it back;
 // if all find their own, no class is listed twice and they write their exponentials there.  Otherwise the wave adds the
 // entries one by one in list order.
-template <int G, int VPL>
-__device__ __forceinline__ void load_logits(const float* __restrict__ row, int sub, int c, bool last, float (&x)[VPL][4]) {
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-        // a vector that begins in the row may end in the next one, whose values are replaced below; behind the last
-        // row there may be nothing
-        const int at = 4 * (sub + G * v);
-        if (!last || at + 4 <= c) {
-            const f4u f = *reinterpret_cast<const f4u*>(row + (at < c ? at : 0));
-            x[v][0] = f.x;
-            x[v][1] = f.y;
-            x[v][2] = f.z;
-            x[v][3] = f.w;
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[v][q] = at + q < c ? row[at + q] : 0.0f;
-        }
-    }
-}
-// the row's columns; the one vector that the row's end cuts is stored by one instruction of its length
-template <int G, int VPL>
-__device__ __forceinline__ void store_grad(float* __restrict__ row, int sub, int c, const float (&g)[VPL][4]) {
-    const int cut = c & 3;
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-        const int at = 4 * (sub + G * v);
-        if (at + 4 <= c) *reinterpret_cast<f4u*>(row + at) = f4u{g[v][0], g[v][1], g[v][2], g[v][3]};
-        if (cut != 0 && at < c && at + 4 > c) {
-            typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
-            typedef float f3u __attribute__((ext_vector_type(3), aligned(4)));
-            if (cut == 1) row[at] = g[v][0];
-            else if (cut == 2) *reinterpret_cast<f2u*>(row + at) = f2u{g[v][0], g[v][1]};
-            else *reinterpret_cast<f3u*>(row + at) = f3u{g[v][0], g[v][1], g[v][2]};
-        }
-    }
-}
-
 // A lane holds NE entries of the list in registers (G NE of them a row); MORE: longer lists, whose other entries are read
 // again by every pass over the list (17 entries on 47 classes: 1.13 ms against 0.48 in registers).
 template <int G, int VPL, int NE, bool MORE>
@@ -148,7 +111,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int t
     const int rows = (int)(base >= a.n ? 0 : std::min<int64_t>(tile, (a.n - base + kRows - 1) / kRows));   // of this group
     const int left = a.c - 4 * sub;                  // columns from the lane's first one on
     auto load_mask = [&](int t) { return t < rows ? (a.mask ? a.mask[base + (int64_t)t * kRows] : 1) : 0; };
-    auto load_row = [&](int t, int m, float (&x)[VPL][4], RawEntry (&e)[NE]) {
+    auto fetch_row = [&](int t, int m, float (&x)[VPL][4], RawEntry (&e)[NE]) {
 #pragma unroll
         for (int u = 0; u < NE; ++u) e[u] = {0u, 0, -1};
 #pragma unroll
@@ -157,7 +120,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int t
             for (int q = 0; q < 4; ++q) x[v][q] = 0.0f;
         if (m != 0) {
             const int64_t i = base + (int64_t)t * kRows;
-            load_logits<G, VPL>(a.logits + i * a.ldx, sub, a.c, i == a.n - 1, x);
+            load_row<G, VPL>(a.logits + i * a.ldx, sub, a.c, i == a.n - 1, x);
 #pragma unroll
             for (int u = 0; u < NE; ++u) e[u] = fetch_entry(a, i, G * u + sub);
         }
@@ -165,7 +128,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int t
     float nx[VPL][4];
     RawEntry ne[NE];
     int nm = load_mask(0);
-    load_row(0, nm, nx, ne);
+    fetch_row(0, nm, nx, ne);
     int nnm = load_mask(1);
     for (int t = 0; t < tile; ++t) {
         if ((int64_t)blockIdx.x * tile * kRows + (int64_t)t * kRows >= a.n) break;      // uniform in the workgroup
@@ -191,7 +154,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int t
                 xm = fmaxf(xm, x[v][q]);
             }
         nm = nnm;
-        load_row(t + 1, nm, nx, ne);
+        fetch_row(t + 1, nm, nx, ne);
         nnm = load_mask(t + 2);
         const float w = (float)m * a.inv_mask_mean;
         xm = lanes_reduce<G, OpMax>(xm);
@@ -290,7 +253,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int t
             for (int v = 0; v < VPL; ++v)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) x[v][q] = any ? (x[v][q] * qs - p[v][q]) * scale : 0.0f;
-            if (live) store_grad<G, VPL>(a.grad + i * a.ldg, sub, a.c, x);
+            if (live) store_row<G, VPL>(a.grad + i * a.ldg, sub, a.c, x);
         }
     }
 }
@@ -411,7 +374,7 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
         return;
     }
     float x[VPL][4];
-    load_logits<G, VPL>(xr, sub, a.c, i == a.n - 1, x);
+    load_row<G, VPL>(xr, sub, a.c, i == a.n - 1, x);
     Listed l;
     if (lister) {
         l = list_entries(a, i, lane, list);
@@ -450,7 +413,7 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) x[j][q] = l.any ? x[j][q] * all : 0.0f;
-        store_grad<G, VPL>(gr, sub, a.c, x);
+        store_row<G, VPL>(gr, sub, a.c, x);
     }
     if (a.stats) {
         first = __float_as_int(wide_reduce<G, OpMinInt>(__int_as_float(first), lds[2]));

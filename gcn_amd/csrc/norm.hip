@@ -9,8 +9,12 @@
 //
 // Both directions are bound by memory: a row is read once, lives in registers between the reduction and the use of
 // its result, and is written once.  A row of f columns belongs to G lanes (G a power of two; a wave holds 64 / G
-// rows) or, past 2048 columns, to a whole workgroup; lane l holds the columns 4 (l + G j) .. + 3, so that an
+// rows) or, past 1024 columns, to a whole workgroup; lane l holds the columns 4 (l + G j) .. + 3, so that an
 // instruction of a group reads 16 G consecutive bytes.  Sums, the maximum and the weight's gradient are float32.
+// Measured, compulsory bytes over time (a large copy: 4.7 TB/s), rows of 1 GB: 8-bit output with residual 4.8 to 5.2 TB/s at
+// 16, 64, 256, 500, 1433, 2048 and 8192 columns (100: 4.0, whose 112 of 128 bytes a row are partial lines), float32 output
+// 4.9 to 5.3, gradients 4.3 to 5.0; past 16,384 columns the registers of a row no longer fit and the gradient falls to 1.4.
+// A wave a row at 1433 columns (eight vectors a lane, two waves a SIMD) ran the gradient at 2.6 instead of 4.7.
 #include <algorithm>
 
 #include "common.h"
@@ -20,6 +24,7 @@
 namespace gcn {
 
 constexpr int kNormMaxF = 32768;
+constexpr int kWaveRowF = 1024;          // wider rows belong to a workgroup each
 // sum or maximum over the G lanes of a row (G <= 64: lanes of one wave; more: the workgroup, through `lds`)
 template <int G, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* lds) {
@@ -76,6 +81,7 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
         }
     }
     const float inv_f = 1.0f / (float)f;
+    const int left = f - 4 * sub;                    // columns from the lane's first one on
     const int64_t base = (int64_t)blockIdx.x * tile * kRows;
     for (int t = 0; t < tile; ++t) {
         const int64_t i = base + (int64_t)t * kRows + threadIdx.x / G;
@@ -83,32 +89,23 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
         const bool live = i < a.n;
         float v[VPL][4], sum = 0.0f;
         const int64_t row = live ? i : a.n - 1;
-        const float* xr = a.x + row * a.ldx;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            const int c = 4 * (sub + G * j);
-            load_cols(xr, c < f ? c : 0, f, v[j]);
-        }
+        const bool last = row == a.n - 1;
+        load_row<G, VPL>(a.x + row * a.ldx, sub, f, last, v);
         if (a.residual) {
-            const float* rr = a.residual + row * a.ldr;
             float r[VPL][4];
+            load_row<G, VPL>(a.residual + row * a.ldr, sub, f, last, r);
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                const int c = 4 * (sub + G * j);
-                load_cols(rr, c < f ? c : 0, f, r[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) {
+            for (int j = 0; j < VPL; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[j][e] += r[j][e];
-                if (live && 4 * (sub + G * j) < f) store_cols(a.h + i * a.ldh, 4 * (sub + G * j), f, v[j]);
-            }
+            if (live) store_row<G, VPL>(a.h + i * a.ldh, sub, f, v);
         }
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
-            if (4 * (sub + G * j) < f) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum = fmaf(v[j][e], v[j][e], sum);
+            for (int e = 0; e < 4; ++e) {
+                v[j][e] = 4 * G * j + e < left ? v[j][e] : 0.0f;
+                sum = fmaf(v[j][e], v[j][e], sum);
             }
         sum = row_reduce<G, false>(sum, lds[2 * (t & 1)]);
         const float ms = sum * inv_f;
@@ -119,18 +116,14 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] * inv * w[j][e];
         if (!a.q) {
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (live && 4 * (sub + G * j) < f) store_cols(a.y + i * a.ldy, 4 * (sub + G * j), f, v[j]);
+            if (live) store_row<G, VPL>(a.y + i * a.ldy, sub, f, v);
             continue;
         }
         float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
-            if (4 * (sub + G * j) < f) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[j][e]));
-            }
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[j][e]));      // 0 past the row's end
         most = row_reduce<G, true>(most, lds[2 * (t & 1) + 1]);
         float scale = fmaxf(most * (1.0f / kE4m3Max), kQuantScaleMin);
         // a row whose mean square or maximum is not finite has no scale: it stands for NaN as a whole
@@ -183,48 +176,42 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_grad_kernel(NormGradArgs a, in
         if (a.w && c < f) load_cols(a.w, c, f, w[j]);
     }
     const float inv_f = 1.0f / (float)f;
+    const int left = f - 4 * sub;                    // columns from the lane's first one on
     const int64_t base = (int64_t)blockIdx.x * tile * kRows;
     for (int t = 0; t < tile; ++t) {
         const int64_t i = base + (int64_t)t * kRows + group;
         if (base + (int64_t)t * kRows >= a.n) break;                         // uniform in the workgroup
         const bool live = i < a.n;
         const int64_t row = live ? i : a.n - 1;
-        const float* dyr = a.dy + row * a.lddy;
-        const float* hr = a.h + row * a.ldh;
+        const bool last = row == a.n - 1;
         const float inv = a.inv[row];
         float dy[VPL][4], h[VPL][4];
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            const int c = 4 * (sub + G * j);
-            load_cols(dyr, c < f ? c : 0, f, dy[j]);
-            load_cols(hr, c < f ? c : 0, f, h[j]);
-        }
+        load_row<G, VPL>(a.dy + row * a.lddy, sub, f, last, dy);
+        load_row<G, VPL>(a.h + row * a.ldh, sub, f, last, h);
         float along = 0.0f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool in = 4 * (sub + G * j) < f;
-                if (in) along = fmaf(dy[j][e] * w[j][e], h[j][e], along);
-                if (in && live) dw[j][e] = fmaf(dy[j][e], h[j][e] * inv, dw[j][e]);
+                const bool in = 4 * G * j + e < left;
+                dy[j][e] = in && live ? dy[j][e] : 0.0f;
+                h[j][e] = in ? h[j][e] : 0.0f;
+                along = fmaf(dy[j][e] * w[j][e], h[j][e], along);
+                dw[j][e] = fmaf(dy[j][e], h[j][e] * inv, dw[j][e]);
             }
         along = row_reduce<G, false>(along, lds[t & 1]);
         const float back = along * inv_f * inv * inv;
         if (a.dx) {
+            float u[VPL][4];
+            if (a.dh) load_row<G, VPL>(a.dh + row * a.lddh, sub, f, last, u);
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                const int c = 4 * (sub + G * j);
-                float o[4];
+            for (int j = 0; j < VPL; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = inv * (dy[j][e] * w[j][e] - h[j][e] * back);
-                if (a.dh) {
-                    float u[4];
-                    load_cols(a.dh + row * a.lddh, c < f ? c : 0, f, u);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] += u[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float o = inv * (dy[j][e] * w[j][e] - h[j][e] * back);
+                    dy[j][e] = a.dh ? o + u[j][e] : o;
                 }
-                if (live && c < f) store_cols(a.dx + i * a.lddx, c, f, o);
-            }
+            if (live) store_row<G, VPL>(a.dx + i * a.lddx, sub, f, dy);
         }
     }
     if (!a.part) return;
@@ -292,7 +279,7 @@ static inline int norm_rows(int64_t f) {
     const int64_t vecs = ceil_div(f, (int64_t)4);
     int g = 4;
     while (g < 64 && g < vecs) g <<= 1;
-    return f <= 2048 ? 256 / g : 1;
+    return f <= kWaveRowF ? 256 / g : 1;
 }
 
 #define GCN_NORM_BY_WIDTH(LAUNCH)              \
@@ -303,7 +290,7 @@ static inline int norm_rows(int64_t f) {
     else if (f <= 256) { LAUNCH(64, 1, 256); } \
     else if (f <= 512) { LAUNCH(64, 2, 256); } \
     else if (f <= 1024) { LAUNCH(64, 4, 256); } \
-    else if (f <= 2048) { LAUNCH(64, 8, 256); } \
+    else if (f <= 2048) { LAUNCH(256, 2, 256); } \
     else if (f <= 4096) { LAUNCH(256, 4, 256); } \
     else if (f <= 8192) { LAUNCH(256, 8, 256); } \
     else if (f <= 16384) { LAUNCH(1024, 4, 1024); } \
