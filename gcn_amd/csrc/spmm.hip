@@ -54,10 +54,8 @@ static int scratch_on_current_device(void** out) {
     return GCN_OK;
 }
 
-constexpr int kStripNnz = 256;       // entries per strip on a matrix large enough to fill the chip with such strips
 constexpr int kStripNnzMin = 16;
 constexpr int kChunkSmall = 64;
-constexpr int kRowCost = 4;          // a row's fixed cost (pointer loads, store) in units of one entry
 constexpr int64_t kStripsWanted = 8192;  // 8 waves on each of the 1024 SIMDs
 
 // A strip is one wave's sequential work (wide operands).  With 256-entry strips a matrix of 10^5

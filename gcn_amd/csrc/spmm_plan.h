@@ -32,6 +32,9 @@ struct gcn_spmm_plan {
 
 namespace gcn {
 
+constexpr int kStripNnz = 256;       // entries per strip on a matrix large enough to fill the chip with such strips
+constexpr int kRowCost = 4;          // a row's fixed cost (pointer loads, store) in units of one entry
+
 struct PlanView {
     int64_t n_strips, n_chunks, chunk_blocks, nnz;
     int split;

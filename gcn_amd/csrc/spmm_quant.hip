@@ -4,12 +4,17 @@
 //   C[i, :] = act(sum_e (a_e s[col_e]) q[col_e, :])        float32 sums, one fused multiply-add an element
 //
 // The product is bound by the rows it gathers: at 256 columns 256 bytes an entry (two 128-byte lines) and the entry's
-// scale, instead of the 1024 bytes of float32 rows.  A wave takes the strips of rows the plan cut, one row after the
-// other.  L lanes hold 16 columns each (one 16-byte load a row), so 64 / L entries of the row are gathered by one
-// instruction; each lane group adds its entries, and at the end of a row the groups are added by exchanging halves: after
-// the exchange over lane distance 32 a lane is left with 8 of its 16 columns, then 4, 2, 1.  64 (column, value)
-// pairs of a row are read by one load each, a lane an entry, with the gather of their scales; the lanes' entries
-// then reach the groups by shuffles.  Long rows are cut at the chunks of the wide dense product and joined in chunk order.
+// scale, instead of the 1024 bytes of float32 rows.  A wave takes a strip of the rows the plan cut.  L lanes hold 16 columns
+// each (one 16-byte load a row), so 64 / L entries are gathered by one instruction; each lane group adds its entries, and at
+// the end of a row the groups are added by exchanging halves: after the exchange over lane distance 32 a lane is left with
+// 8 of its 16 columns, then 4, 2, 1.  Long rows are cut at the chunks of the wide dense product and joined in chunk order.
+// Measured (R-MAT, 32 entries a row; rows gathered + compulsory bytes over time; random row gathers end at 7.5 TB/s):
+// 2^20 nodes x 256: 1.29 ms, 7.5 TB/s (float32 rows: 3.92 ms); x 512: 2.54 (8.34); x 128: 0.81 (1.93); x 16: 0.58 (0.56).
+// 2^24 nodes x 256: 28.5 ms (74.6), x 128: 18.9 (39.0), x 64: 18.1 (20.0), x 16: 16.7 (10.7): there the 64 MB of scales no
+// longer stay in the L2s and every entry pays a line for its scale, so rows of 64 columns and fewer are for small graphs.
+// Steps tried on 2^20 x 256 / 2^24 x 256: a row after the other, every row's loads drained before the next row's
+// 1.62 / 33.8 ms; the stream below with 4 steps in flight 1.38 / 28.8, with 8 (4 waves a SIMD) 1.55 / 30.3, with 2 and 6 waves
+// a SIMD 1.29 / 28.5; non-temporal row loads 1.95 / 32.3 (the hubs' rows leave the L2).
 #include <algorithm>
 
 #include "common.h"
@@ -77,42 +82,82 @@ __device__ __forceinline__ int add_groups(float (&acc)[16], int lane) {
     return offset;
 }
 
-// sums of the entries k0 .. k1 - 1, this lane's 16 columns, before the groups are added
-template <int L>
-__device__ __forceinline__ void accumulate_quant(int64_t k0, int64_t k1, const int32_t* __restrict__ indices,
-                                                 const float* __restrict__ vals, const uint8_t* __restrict__ q, uint32_t ldq,
-                                                 const float* __restrict__ scales, int lane, int64_t piece,
-                                                 float (&acc)[16]) {
-    constexpr int P = 64 / L;              // entries a step gathers
-    constexpr int U = 4;                   // steps in flight
+// A run of `total` consecutive entries from k0 on, holding whole rows one after the other: row number x of the run ends
+// before entry row_end(x) of it (non-decreasing, the last one `total`); finish(x) takes the sums of row x out of acc.
+// The entries are one stream, whatever rows they belong to: lane l holds (column, weight) of entry 64 b + l of batch b, the
+// pairs are fetched two batches and the scales one batch ahead, and step s of a batch gathers entries s P .. s P + P - 1, one
+// a lane group, U steps in flight while the U before are added.  A step that a row ends in is added once for every row it
+// touches, the pieces and weights of other rows replaced by zeros (not multiplied by zero: they may be NaN).
+template <int L, int U, class RowEnd, class Finish>
+__device__ __forceinline__ void stream_quant(int64_t k0, int total, const int32_t* __restrict__ indices,
+                                             const float* __restrict__ vals, const uint8_t* __restrict__ q, uint32_t ldq,
+                                             const float* __restrict__ scales, int lane, int64_t piece, int rows,
+                                             RowEnd row_end, Finish finish, float (&acc)[16]) {
+    constexpr int P = 64 / L, C = L / U;
     const int group = lane / L;
-    for (int64_t k = k0; k < k1; k += 64) {
-        // lanes past the end repeat the last entry with weight 0: its row is read anyway
-        const int64_t e = k + lane < k1 ? k + lane : k1 - 1;
-        const int32_t col = indices[e];
-        float w = vals[e] * scales[col];
-        if (k + lane >= k1) w = 0.0f;
-        const int n = (int)(k1 - k < 64 ? k1 - k : 64);
-        const int steps = (n + P - 1) / P;
-        for (int s = 0; s < steps; s += U) {
-            uint4 raw[U];
-            float ws[U];
+    int row = 0, begin = 0, end = row_end(0);            // the row in work: entries begin .. end - 1
+    if (total > 0) {
+        auto entry = [&](int t) { return k0 + (t < total ? t : total - 1); };      // past the end: the last one again
+        auto gather = [&](uint4 (&raw)[U], int32_t col, int chunk) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int from = min((s + u) * P + group, 63);
-                const int32_t c = __shfl(col, from);
-                ws[u] = __shfl(w, from);
-                if (s + u >= steps) ws[u] = 0.0f;
-                raw[u] = *reinterpret_cast<const uint4*>(q + (uint64_t)(uint32_t)c * ldq + piece);
+                const uint32_t c = (uint32_t)__shfl(col, (chunk * U + u) * P + group);
+                raw[u] = *reinterpret_cast<const uint4*>(q + (uint64_t)c * ldq + piece);
             }
+        };
+        int32_t col = indices[entry(lane)], col1 = indices[entry(64 + lane)];
+        float val1 = vals[entry(64 + lane)];
+        float w = vals[entry(lane)] * scales[col];
+        uint4 raw[U];
+        gather(raw, col, 0);
+        for (int t0 = 0; t0 < total; t0 += 64) {
+            const float scale1 = scales[col1];
+            const int32_t col2 = indices[entry(t0 + 128 + lane)];
+            const float val2 = vals[entry(t0 + 128 + lane)];
+#pragma unroll 1
+            for (int c = 0; c < C; ++c) {
+                uint4 next[U];
+                const int t1 = t0 + (c + 1) * U * P;                 // first entry of the next chunk
+                if (t1 < total) gather(next, c + 1 < C ? col : col1, c + 1 < C ? c + 1 : 0);
 #pragma unroll
-            for (int u = 0; u < U; ++u) add_piece(raw[u], ws[u], acc);
+                for (int u = 0; u < U; ++u) {
+                    const int from = t0 + (c * U + u) * P, to = from + P;
+                    const float ws = __shfl(w, (c * U + u) * P + group);
+                    if (from < total) {
+                        if (begin <= from && end > to) {
+                            add_piece(raw[u], ws, acc);
+                        } else {
+                            const int idx = from + group;
+                            for (;;) {
+                                if (end > begin && end > from) {
+                                    const bool in = idx >= begin && idx < end;
+                                    const uint4 mine = {in ? raw[u].x : 0u, in ? raw[u].y : 0u, in ? raw[u].z : 0u, in ? raw[u].w : 0u};
+                                    add_piece(mine, in ? ws : 0.0f, acc);
+                                }
+                                if (end > to || row == rows) break;
+                                finish(row);
+                                begin = end;
+                                ++row;
+                                if (row < rows) end = row_end(row);
+                                if (row == rows || begin >= to) break;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = next[u];
+            }
+            col = col1;
+            w = val1 * scale1;
+            col1 = col2;
+            val1 = val2;
         }
     }
+    for (; row < rows; ++row) finish(row);               // empty rows at the end
 }
 
-template <int L>
-__global__ __launch_bounds__(kBlock) void spmm_quant_kernel(PlanView pv, const int64_t* __restrict__ indptr,
+template <int L, int U>
+__global__ __launch_bounds__(kBlock, 6) void spmm_quant_kernel(PlanView pv, const int64_t* __restrict__ indptr,
                                                             const int32_t* __restrict__ indices,
                                                             const float* __restrict__ vals, int f,
                                                             const uint8_t* __restrict__ q, uint32_t ldq,
@@ -125,23 +170,27 @@ __global__ __launch_bounds__(kBlock) void spmm_quant_kernel(PlanView pv, const i
     const int64_t piece = col0 < f ? col0 : (int64_t)blockIdx.y * 16 * L;
     const int64_t block = blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    auto finish = [&](float (&acc)[16], float* row, bool vec, bool act) {
+    auto store = [&](float (&acc)[16], float* row, bool vec, bool act) {
         const int at = col0 + add_groups<L>(acc, lane);
-        if (L < 4 && (lane & 3 & ~(L - 1))) return;                 // L = 1, 2: the groups past the fourth hold the same sum
+        if (!(L < 4 && (lane & 3 & ~(L - 1)))) {                    // L = 1, 2: the groups past the fourth hold the same sum
 #pragma unroll
-        for (int i = 0; i < kLeft; ++i)
-            if (act) acc[i] = acc[i] > 0.0f ? acc[i] : 0.0f;
+            for (int i = 0; i < kLeft; ++i)
+                if (act) acc[i] = acc[i] > 0.0f ? acc[i] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < kLeft; i += 4) {
-            if (kLeft >= 4 && vec && at + i + 4 <= f) {
-                *reinterpret_cast<float4*>(row + at + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-            } else {
+            for (int i = 0; i < kLeft; i += 4) {
+                if (kLeft >= 4 && vec && at + i + 4 <= f) {
+                    *reinterpret_cast<float4*>(row + at + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4 && i + e < kLeft; ++e)
-                    if (at + i + e < f) row[at + i + e] = acc[i + e];
+                    for (int e = 0; e < 4 && i + e < kLeft; ++e)
+                        if (at + i + e < f) row[at + i + e] = acc[i + e];
+                }
             }
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
     };
+    float acc[16] = {};
     if (block < pv.chunk_blocks) {
         const int64_t chunk = block * (kBlock / 64) + wave;
         if (chunk >= pv.n_chunks) return;
@@ -149,21 +198,35 @@ __global__ __launch_bounds__(kBlock) void spmm_quant_kernel(PlanView pv, const i
         const int r = pv.long_row[li];
         const int64_t k0 = indptr[r] + (chunk - pv.long_chunk[li]) * (int64_t)pv.chunk_len;
         const int64_t row_end = indptr[r + 1];
-        const int64_t k1 = k0 + pv.chunk_len < row_end ? k0 + pv.chunk_len : row_end;
-        float acc[16] = {};
-        accumulate_quant<L>(k0, k1, indices, vals, q, ldq, scales, lane, piece, acc);
-        finish(acc, part + chunk * ldp, true, false);               // partial rows: 16-byte aligned, pitch a multiple of 4
+        const int total = (int)(k0 + pv.chunk_len < row_end ? pv.chunk_len : row_end - k0);
+        // partial rows: 16-byte aligned, pitch a multiple of 4
+        stream_quant<L, U>(k0, total, indices, vals, q, ldq, scales, lane, piece, 1, [&](int) { return total; },
+                           [&](int) { store(acc, part + chunk * ldp, true, false); }, acc);
         return;
     }
     const int64_t strip = (block - pv.chunk_blocks) * (kBlock / 64) + wave;
     if (strip >= pv.n_strips) return;
-    const int r_hi = pv.strip_row[strip + 1];
-    for (int r = pv.strip_row[strip]; r < r_hi; ++r) {
-        const int64_t k0 = indptr[r], k1 = indptr[r + 1];
-        if (k1 - k0 > pv.split) continue;                           // summed chunk-wise
-        float acc[16] = {};
-        accumulate_quant<L>(k0, k1, indices, vals, q, ldq, scales, lane, piece, acc);
-        finish(acc, c + (int64_t)r * ldc, c_vec != 0, relu != 0);
+    // A strip has at most 64 rows: lane l keeps the end of row r_lo + l,
+    // counted from the strip's first entry.  Rows that are summed chunk-wise cut the strip's entries into runs.
+    static_assert(kStripNnz / kRowCost <= 64, "a strip's rows are held one a lane");
+    const int r_lo = pv.strip_row[strip], n_rows = pv.strip_row[strip + 1] - r_lo;
+    if (n_rows == 0) return;
+    const int64_t base = indptr[r_lo];
+    const int mine = lane < n_rows ? lane : n_rows - 1;
+    const int64_t len = indptr[r_lo + mine + 1] - indptr[r_lo + mine];
+    const int ends = (int)min(indptr[r_lo + mine + 1] - base, (int64_t)0x7fffffff);
+    uint64_t cut = __ballot(lane < n_rows && len > pv.split);
+    for (int first = 0; first < n_rows;) {
+        const int next = cut ? __builtin_ctzll(cut) : n_rows;      // the next row that is summed chunk-wise
+        if (next > first) {
+            const int at = first ? __builtin_amdgcn_readlane(ends, first - 1) : 0;
+            const int total = __builtin_amdgcn_readlane(ends, next - 1) - at;
+            stream_quant<L, U>(base + at, total, indices, vals, q, ldq, scales, lane, piece, next - first,
+                               [&](int x) { return __builtin_amdgcn_readlane(ends, first + x) - at; },
+                               [&](int x) { store(acc, c + (int64_t)(r_lo + first + x) * ldc, c_vec != 0, relu != 0); }, acc);
+        }
+        first = next + 1;
+        cut &= cut - 1;
     }
 }
 
@@ -217,16 +280,16 @@ int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, con
     const int relu = (flags & GCN_RELU) ? 1 : 0;
     const int c_vec = (ldc % 4 == 0 && aligned16(c)) ? 1 : 0;
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[0], st));
-#define GCN_QUANT_GO(L)                                                                                                  \
-    spmm_quant_kernel<L><<<dim3((unsigned)grid, (unsigned)ceil_div(f, (int64_t)16 * L)), kBlock, 0, st>>>(               \
+#define GCN_QUANT_GO(L, U)                                                                                                \
+    spmm_quant_kernel<L, U><<<dim3((unsigned)grid, (unsigned)ceil_div(f, (int64_t)16 * L)), kBlock, 0, st>>>(               \
         pv, indptr, indices, vals, (int)f, q, (uint32_t)ldq, scales, c, ldc, c_vec, part, ldp, relu)
-    if (f <= 16) GCN_QUANT_GO(1);
-    else if (f <= 32) GCN_QUANT_GO(2);
-    else if (f <= 64) GCN_QUANT_GO(4);
-    else if (f <= 128) GCN_QUANT_GO(8);
-    else if (f <= 256) GCN_QUANT_GO(16);
-    else if (f <= 512) GCN_QUANT_GO(32);
-    else GCN_QUANT_GO(64);                                           // wider rows: ranges of 1024 columns
+    if (f <= 16) GCN_QUANT_GO(1, 1);
+    else if (f <= 32) GCN_QUANT_GO(2, 1);
+    else if (f <= 64) GCN_QUANT_GO(4, 2);
+    else if (f <= 128) GCN_QUANT_GO(8, 2);
+    else if (f <= 256) GCN_QUANT_GO(16, 2);
+    else if (f <= 512) GCN_QUANT_GO(32, 2);
+    else GCN_QUANT_GO(64, 2);                                           // wider rows: ranges of 1024 columns
 #undef GCN_QUANT_GO
     GCN_LAUNCH_CHECK();
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[1], st));
