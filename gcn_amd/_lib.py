@@ -117,6 +117,7 @@ SIGNATURES = {
     'gcn_adam_f32': [_i64, _vp, _vp, _vp, _vp, _f32, _vp, _f32, _f32, _f32, _f32, _vp],
     'gcn_gemm_tn_f32': [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_size_t, _vp],
     'gcn_quant_pitch': [_i64, _pi64],
+    'gcn_quant_dense_f32': [_i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp],
     'gcn_rms_norm_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp],
     'gcn_rms_norm_grad_workspace_bytes': [_i64, _i64, _psz],
     'gcn_rms_norm_grad_f32': [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],

@@ -343,6 +343,7 @@ int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const fl
     if (n == 0) return GCN_OK;
     if ((y != nullptr) == (q != nullptr)) return fail(GCN_ERR_BAD_ARG, "one of the outputs y and q is wanted");
     if (!x || !inv || (residual && !h)) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    if (y && residual && y == h) return fail(GCN_ERR_BAD_ARG, "y and h are two outputs: they need memory of their own");
     NormArgs a = {n, (int)f, x, ldx, residual, ldr, weight, eps, h, ldh, inv, y, ldy, q, ldq, scales};
     const int tile = norm_tile(n, f);
     const int64_t blocks = ceil_div(n, (int64_t)norm_rows(f) * tile);

@@ -230,6 +230,23 @@ __global__ __launch_bounds__(kBlock, 6) void spmm_quant_kernel(PlanView pv, cons
     }
 }
 
+// y <- the float32 values an 8-bit matrix stands for, four columns a thread
+__global__ __launch_bounds__(kBlock) void quant_dense_kernel(int64_t n_rows, int f, const uint8_t* __restrict__ q, int64_t ldq,
+                                                             const float* __restrict__ scales, float* __restrict__ y,
+                                                             int64_t ldy) {
+    const int64_t per_row = (f + 3) / 4, total = n_rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < total; i += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = i / per_row;
+        const int c = 4 * (int)(i - r * per_row);
+        const int word = *reinterpret_cast<const int*>(q + r * ldq + c);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+        const float s = scales[r], v[4] = {s * lo.x, s * lo.y, s * hi.x, s * hi.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < f) y[r * ldy + c + e] = v[e];
+    }
+}
+
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace gcn
@@ -237,6 +254,19 @@ static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 using namespace gcn;
 
 extern "C" {
+
+int gcn_quant_dense_f32(int64_t n_rows, int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* y, int64_t ldy,
+                        void* stream) {
+    if (n_rows < 0 || f < 1 || f > 32768) return fail(GCN_ERR_BAD_ARG, "an 8-bit row holds 1 to 32768 columns: f=%lld", (long long)f);
+    if (ldy < f || ldq < (f + 15) / 16 * 16 || ldq % 16 != 0) return fail(GCN_ERR_BAD_ARG, "bad pitch");
+    if (n_rows == 0) return GCN_OK;
+    if (!q || !scales || !y) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    if (!aligned16(q)) return fail(GCN_ERR_BAD_ARG, "8-bit rows must be 16-byte aligned");
+    const int64_t blocks = std::min<int64_t>(ceil_div(n_rows * ((f + 3) / 4), (int64_t)kBlock), 1 << 16);
+    quant_dense_kernel<<<(unsigned)blocks, kBlock, 0, (hipStream_t)stream>>>(n_rows, (int)f, q, ldq, scales, y, ldy);
+    GCN_LAUNCH_CHECK();
+    return GCN_OK;
+}
 
 int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, const int32_t* indices, const float* vals,
                            int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* c, int64_t ldc, int flags,

@@ -1005,6 +1005,17 @@ class QuantRows(object):
         rows.scales = torch.empty(n_rows, dtype=torch.float32, device=device)
         return rows
 
+    def dense(self, out=None):
+        """The float32 matrix these rows stand for."""
+        with _on_device(self.data, out):
+            if out is None:
+                out = self.scales.new_empty((self.n_rows, self.f))
+            else:
+                _check_out(out, self.n_rows, self.f)
+            _lib.call('gcn_quant_dense_f32', self.n_rows, self.f, _at(self.data), self.ld, _at(self.scales), _at(out), _ld(out),
+                      _raw_stream())
+        return out
+
     def rows(self, begin, end):
         """Rows begin .. end - 1 as QuantRows over the same memory."""
         return QuantRows(end - begin, self.f, self.data[begin:end], self.scales[begin:end])
@@ -1014,7 +1025,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=False, out=None, sum
     """``(y, h, inv)`` with ``h = x + residual`` (``x`` itself without a residual), ``inv = 1 / sqrt(mean(h^2) + eps)``
     of every row and ``y = h * inv * weight``: float32, or QuantRows with ``quant``.  One pass over the rows.
     ``out``: where ``y`` goes (a float32 view, or QuantRows); ``sum_out``: where ``h`` goes, which may be ``x`` or
-    ``residual`` itself.  A row holds at most 32768 columns.  ``h`` and ``inv`` are what ``rms_norm_grad`` wants."""
+    ``residual`` itself (``y`` and ``h`` need memory of their own).  A row holds at most 32768 columns.  ``h`` and
+    ``inv`` are what ``rms_norm_grad`` wants."""
     with _on_device(x, weight, residual, sum_out):
         x = _matrix(x)
         n, f = x.shape
@@ -1081,7 +1093,8 @@ def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
 def spmm_quant(a, q, relu=False, out=None):
     """``a @ B`` (optionally with ReLU) for the matrix B that the QuantRows ``q`` stand for, gathering their 8-bit rows.
     float32 sums in a fixed order (not the serial order of ``spmm``).  The workspace of long rows belongs to the call, so
-    products on several streams, or recorded in several graphs, do not share one."""
+    products on several streams, or recorded in several graphs, do not share one; the plan of ``a`` is made at the first
+    product (touch ``a.plan`` before recording)."""
     if not isinstance(q, QuantRows):
         raise ValueError('spmm_quant takes QuantRows')
     with _on_device(q.data, a.indptr, out):

@@ -533,12 +533,15 @@ int gcn_adam_f32(int64_t n, float* param, const float* grad, float* m, float* v,
  * gcn_quant_pitch: the pitch to allocate for f <= 32768 columns -- a power of two up to 128 bytes, then a multiple
  * of 64, so that a gathered row straddles no line it need not touch. */
 int gcn_quant_pitch(int64_t f, int64_t* pitch_bytes);
+/* y [n_rows x f] <- the float32 matrix such rows stand for. */
+int gcn_quant_dense_f32(int64_t n_rows, int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* y, int64_t ldy,
+                        void* stream);
 
 /* Root-mean-square norm of every row, with the residual's addition in front of it:
  *   h = x + residual (x itself if residual is NULL),  inv = 1 / sqrt(mean_c h_c^2 + eps),  y_c = h_c * inv * weight_c
  * (weight NULL: all ones), f <= 32768 columns.  Written: h (only with a residual; may be x or residual itself), inv
  * [n] (what gcn_rms_norm_grad_f32 wants), and one of
- *   y  [n x f] float32 (may be x or residual itself where that is not also h), or
+ *   y  [n x f] float32 (may be x or residual itself, but not h), or
  *   q, scales: y as 8-bit rows, scales[r] = max(max_c |y_c| / 448, 2^-120), q_c = e4m3(y_c / scales[r]) rounded to
  *   nearest even, the bytes up to the next multiple of 16 zero.  A row whose mean square or maximum is not finite gets
  *   the scale NaN and stands for NaN as a whole.

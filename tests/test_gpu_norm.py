@@ -217,6 +217,27 @@ def test_another_stream_and_a_graph():
         assert torch.equal(gdx, dx) and torch.equal(gdw, dw)
 
 
+def test_element_offsets_past_32_bits():
+    """2.2 million rows of 1000 columns: offsets past 2^31 elements; the last rows against the formula, forward (float32 and
+    8 bits) and backward."""
+    import torch
+    from gcn_amd import sparse
+    n, f, m = 2200000, 1000, 20
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip('needs 60 GB of free device memory')
+    x = torch.empty((n, f), device='cuda').normal_(generator=torch.Generator('cuda').manual_seed(1))
+    w = torch.rand(f, device='cuda')
+    y, h, inv = sparse.rms_norm(x, w)
+    ry = _reference(x[-m:], None, w, 1e-6)[0]
+    assert bool(((y[-m:].double() - ry).abs() <= 70 * U * ry.abs()).all())
+    dx, _ = sparse.rms_norm_grad(y, h, w, inv)
+    small, _ = sparse.rms_norm_grad(y[-m:], x[-m:], w, inv[-m:])
+    assert torch.equal(dx[-m:], small)
+    del y, dx
+    q, _, _ = sparse.rms_norm(x, w, quant=True)
+    _check_rows(q.rows(n - m, n), ry, x)
+
+
 def test_refusals():
     import torch
     from gcn_amd import sparse
@@ -225,7 +246,7 @@ def test_refusals():
     bad = [lambda: sparse.rms_norm(x, torch.ones(5, device='cuda')), lambda: sparse.rms_norm(x, w, residual=x[:3]),
            lambda: sparse.rms_norm(x.cpu(), w), lambda: sparse.rms_norm(x, w.cpu()), lambda: sparse.rms_norm(x[0], w),
            lambda: sparse.rms_norm(x, w, eps=-1.0), lambda: sparse.rms_norm(x, w, eps=float('nan')),
-           lambda: sparse.rms_norm(x, w, sum_out=x), lambda: sparse.rms_norm(x, w, quant=True, out=x),
+           lambda: sparse.rms_norm(x, w, sum_out=x), lambda: sparse.rms_norm(x, w, residual=x, out=x, sum_out=x), lambda: sparse.rms_norm(x, w, quant=True, out=x),
            lambda: sparse.rms_norm(x, w, out=x[:3]), lambda: sparse.rms_norm(torch.ones((2, 32769), device='cuda')),
            lambda: sparse.rms_norm(torch.ones((2, 0), device='cuda')),
            lambda: sparse.rms_norm_grad(x, x[:3], w, torch.ones(3, device='cuda')),

@@ -170,6 +170,22 @@ def test_norm_then_product_is_the_product_of_the_rows_it_stands_for():
     _check(a, q, sparse.spmm_quant(a, q))
 
 
+@pytest.mark.parametrize('f', [1, 3, 16, 50, 129, 1025])
+def test_dense_form(f):
+    """scale times value, one rounding: the same bits as torch's product of the same float32 numbers."""
+    import torch
+    from gcn_amd import sparse
+    q = _rows(37, f, f)
+    want = q.data[:, :f].contiguous().view(torch.float8_e4m3fn).float() * q.scales[:, None]
+    assert torch.equal(q.dense(), want)
+    room = torch.full((39, f + 5), 2.0, device='cuda')
+    q.dense(out=room[1:38, 3:3 + f])
+    assert torch.equal(room[1:38, 3:3 + f], want) and float(room.sum()) == pytest.approx(
+        float(want.double().sum()) + 2.0 * (room.numel() - want.numel()), rel=1e-4, abs=1.0)
+    assert sparse.QuantRows.empty(0, f, 'cuda').dense().shape == (0, f)
+    assert torch.equal(q.rows(5, 9).dense(), want[5:9])
+
+
 def test_refusals():
     import torch
     from gcn_amd import sparse

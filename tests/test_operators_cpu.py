@@ -32,7 +32,7 @@ def test_norm_refuses():
     assert _norm(n=0) == 0
     for bad in (dict(n=-1), dict(f=0), dict(f=32769, ldx=32769, ldy=32769), dict(n=(1 << 32) + 1), dict(ldx=5),
                 dict(ldy=5), dict(r=P, ldr=5, h=P), dict(r=P, ldr=6, h=P, ldh=5), dict(r=P, ldr=6, h=None),
-                dict(x=None), dict(inv=None), dict(y=None), dict(q=P, ldq=16, scales=P), dict(eps=-1.0),
+                dict(x=None), dict(inv=None), dict(y=None), dict(r=P, ldr=6, h=P), dict(q=P, ldq=16, scales=P), dict(eps=-1.0),
                 dict(eps=float('nan')), dict(y=None, q=P, ldq=16, scales=None), dict(y=None, q=P, ldq=8, scales=P),
                 dict(y=None, q=P, ldq=24, scales=P), dict(y=None, q=P + 8, ldq=16, scales=P)):
         assert _norm(**bad) == BAD, bad
@@ -104,6 +104,11 @@ def test_activation_gradient_refuses():
 
 def test_quant_product_refuses():
     lib = _lib()
+    assert lib.gcn_quant_dense_f32(0, 4, None, 16, None, None, 4, None) == 0
+    for n, f, q, ldq, s, y, ldy in ((-1, 4, P, 16, P, P, 4), (2, 0, P, 16, P, P, 4), (2, 4, P, 8, P, P, 4), (2, 4, P, 24, P, P, 4),
+                                    (2, 4, P, 16, P, P, 3), (2, 4, None, 16, P, P, 4), (2, 4, P, 16, None, P, 4),
+                                    (2, 4, P, 16, P, None, 4), (2, 4, P + 8, 16, P, P, 4), (2, 17, P, 16, P, P, 17)):
+        assert lib.gcn_quant_dense_f32(n, f, q, ldq, s, y, ldy, None) == BAD
     assert lib.gcn_spmm_csr_quant_f32(None, P, P, P, 4, P, 16, P, P, 4, 0, None, 0, None) == BAD
 
 
