@@ -2018,7 +2018,8 @@ int gcn_spmm_csr_packed_f32(const gcn_spmm_plan* plan, const int64_t* indptr, co
     GCN_LAUNCH_CHECK();
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[1], st));
     if (lt.n_chunks > 0)
-        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu, c_vec, st)) return rc;
+        // the join stores whole vectors only where they end with the row: the columns behind a row are the caller's
+        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu, c_vec && f % 4 == 0, st)) return rc;
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[2], st));
     return GCN_OK;
 }

@@ -120,6 +120,21 @@ def test_empty_matrices_and_one_entry():
     _check(a, q, sparse.spmm_quant(a, q))
 
 
+@pytest.mark.parametrize('f', [33, 130])
+def test_joined_long_rows_leave_the_columns_behind_them(f):
+    """Rows longer than the split, a width that is no multiple of 4, into a slice of a wider matrix with 16-byte aligned
+    rows: the packed and the 8-bit product alike write their columns only."""
+    import torch
+    from gcn_amd import sparse
+    a = _matrix(6, 500, [4000, 3, 2500, 0, 1100, 9], 3)
+    b = torch.randn((500, f), device='cuda') * (torch.rand((500, f), device='cuda') < 0.5)
+    packed, q = sparse.pack_rows(b), sparse.rms_norm(b, quant=True)[0]
+    for product in (lambda out: sparse.spmm_packed(a, packed, out=out), lambda out: sparse.spmm_quant(a, q, out=out)):
+        room = torch.full((6, f + 7 - (f + 7) % 4 + 4), 5.0, device='cuda')
+        product(room[:, :f])
+        assert bool((room[:, f:] == 5.0).all()) and torch.equal(room[:, :f], product(None))
+
+
 def test_element_offsets_past_32_bits():
     """9 million rows of 512 bytes: a byte offset past 2^32 in the operand; the last rows are gathered."""
     import torch
