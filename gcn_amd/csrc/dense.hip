@@ -664,7 +664,15 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
                                                                float* __restrict__ c, int64_t ldc, int relu,
                                                                const float* __restrict__ gate, int64_t ldg,
                                                                float divisor, InMask im, OutDrop od, int raster,
-                                                               EpiArgs ep, int64_t m, int64_t n, int k) {
+                                                               EpiArgs ep, int64_t m, int64_t n, int k, int k_cut) {
+    if (RAGGED && k_cut > 0) {                       // the bare partial product of the k range that grid z names
+        const int from = (int)blockIdx.z * k_cut;
+        a += from;
+        b += TRANS_B ? (int64_t)from : (int64_t)from * ldb;
+        c += (int64_t)blockIdx.z * m * n;
+        k = min(k - from, k_cut);
+        n_ktiles = (k - 1) / 32;
+    }
     constexpr int kBM = 128, BN = 128, kBK = 32, MT = 2, NT = 2;
     constexpr int kAPitch = kBK + 4, kBPitch = BN + 4;
     __shared__ __attribute__((aligned(16))) float as[kBM * kAPitch];
@@ -835,10 +843,15 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
         }
     };
 
-    load_stage(0, 0);
+    if (RAGGED && n_ktiles == 0)
+        load_tail(0);
+    else
+        load_stage(0, 0);
     store_tile();
     __syncthreads();
-    if (RAGGED) {
+    if (RAGGED && n_ktiles == 0) {
+        compute(std::true_type{});
+    } else if (RAGGED) {
         int a_k = 0, b_k = 0;
         for (int t = 1; t <= n_ktiles; ++t) {
             a_k += kBK * 4;
@@ -1049,7 +1062,7 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
         const int raster = n / 128 >= 16 ? 1 : 0;
 #define GCN_PANELS_GO(TB, EPI, AM)                                                                                \
     gemm_panels_kernel<TB, EPI, AM><<<grid, kBlock, 0, st>>>((int)panels, (int)(k / 32), a, lda, b, ldb, c, ldc, relu, gate, \
-                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster, ep, m, n, (int)k)
+                                                             ldg, divisor, im, out_drop ? out_drop_ready(*out_drop) : no_drop, raster, ep, m, n, (int)k, 0)
         if (im.bits) {
             GCN_PANELS_GO(false, kEpiPlain, true);
         } else if (layer) {
@@ -1103,7 +1116,7 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
 #define GCN_RAGGED_GO(TB)                                                                                           \
     gemm_panels_kernel<TB, kEpiLayer, false, true><<<grid, kBlock, 0, st>>>(                                        \
         (int)panels, (int)((k - 1) / 32), a, lda, b, ldb, c, ldc, 0, nullptr, 0, 1.0f, kNoInMask, no_drop, col_tiles >= 16, ep, m, \
-        n, (int)k)
+        n, (int)k, 0)
         if (trans_b)
             GCN_RAGGED_GO(true);
         else
@@ -1141,13 +1154,17 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
     return GCN_OK;
 }
 
-// A layer's product of few tiles and a long k: the k ranges of the cuts run side by side, at least 64 deep and a multiple
-// of the 32-deep stage, as many as give the chip's 768 workgroup slots one each.
+// A layer's product of few tiles and a long k: the k ranges of the cuts run side by side, a multiple of the 32-deep stage,
+// as many as give the chip's 768 workgroup slots one each, at least 64 deep (128 where there are tiles for a quarter of
+// the compute units: the join costs more there than the shorter walk saves; 4934 x 214 x 437 44.6 -> 35.5 us uncut).
+static int64_t layer_tiles(int64_t m, int64_t n) {
+    return ceil_div(m, (int64_t)128) * ceil_div(n, (int64_t)(n <= 32 ? 32 : n <= 64 ? 64 : 128));
+}
 static int64_t layer_cut_k(int64_t k, int64_t cuts) { return align_up(ceil_div(k, cuts), 32); }
 static int64_t layer_cuts(int64_t m, int64_t n, int64_t k) {
     if (m == 0 || n == 0 || k < 128) return 1;
-    const int64_t tiles = ceil_div(m, (int64_t)128) * ceil_div(n, (int64_t)(n <= 32 ? 32 : n <= 64 ? 64 : 128));
-    const int64_t cuts = std::min<int64_t>(std::min<int64_t>(768 / tiles, k / 64), 64);
+    const int64_t tiles = layer_tiles(m, n);
+    const int64_t cuts = std::min<int64_t>(std::min<int64_t>(768 / tiles, k / (tiles <= 64 ? 64 : 128)), 64);
     return cuts > 1 ? ceil_div(k, layer_cut_k(k, cuts)) : 1;
 }
 
@@ -1155,9 +1172,22 @@ template <int BN>
 static int launch_cuts(int64_t m, int64_t n, int64_t k, int64_t cuts, const float* a, int64_t lda, const float* b, int64_t ldb,
                        int trans_b, float* part, hipStream_t st) {
     const int64_t tiles_m = ceil_div(m, (int64_t)128), tiles_n = ceil_div(n, (int64_t)BN);
-    const OutDrop od = {0, 1.0f, 0, 0, nullptr, 0, 0};
-    const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)cuts);
+    const OutDrop od = {0, 1.0f, 0, 0, nullptr, 0, 0, nullptr, 0};
     const int64_t k_cut = layer_cut_k(k, cuts);
+    if (BN == 128 && ragged_form_fits(m, n, k, lda, ldb, trans_b, n)) {
+        const dim3 grid((unsigned)(8 * tiles_n), (unsigned)ceil_div(tiles_m, (int64_t)8), (unsigned)cuts);
+#define GCN_RAGGED_GO(TB)                                                                                       \
+    gemm_panels_kernel<TB, kEpiLayer, false, true><<<grid, kBlock, 0, st>>>((int)tiles_m, 0, a, lda, b, ldb, part, n, 0, nullptr, 0, \
+                                                                            1.0f, kNoInMask, od, 0, kNoEpi, m, n, (int)k, (int)k_cut)
+        if (trans_b)
+            GCN_RAGGED_GO(true);
+        else
+            GCN_RAGGED_GO(false);
+#undef GCN_RAGGED_GO
+        GCN_LAUNCH_CHECK();
+        return GCN_OK;
+    }
+    const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)cuts);
 #define GCN_CUTS_GO(TB)                                                                                                \
     gemm_mfma_kernel<128, BN, TB, 32, true><<<grid, kBlock, 0, st>>>(m, n, k, a, lda, b, ldb, part, n, 0, tiles_m, \
                                                                      tiles_n, nullptr, 0, 1.0f, od, kNoInMask, kNoEpi, k_cut)
@@ -1652,8 +1682,10 @@ int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64
             return rc;
         return launch_join_splits(m, n, cuts, (const float*)workspace, ep, c, ldc, st);
     }
+    // fewer than four 128-column tiles a compute unit: tiles half as wide balance better (20,000 x 512 x 512 168 -> 129 us;
+    // 71,428 x 208 x 355, 1674 tiles, keeps the wide ones: 158 against 167)
     if (n <= 32) return launch_gemm<128, 32>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
-    if (n <= 64) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
+    if (n <= 64 || layer_tiles(m, n) < 1024) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
     return launch_gemm<128, 128>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
 }
 
