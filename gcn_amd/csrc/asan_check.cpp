@@ -33,6 +33,11 @@ static void size_queries() {
         EXPECT(gcn_gemm_tn_workspace_bytes(n, 256, 256, &bytes) == GCN_OK);
         EXPECT(gcn_gemm_tn_workspace_bytes(n, 7, 16, &bytes) == GCN_OK);
         EXPECT(gcn_loss_summary_workspace_bytes(n, 1433 * 16 + 16 * 7, &bytes) == GCN_OK);
+        for (int64_t f : {1ll, 16ll, 1433ll, 32768ll}) {
+            EXPECT(gcn_rms_norm_grad_workspace_bytes(n, f, &bytes) == GCN_OK && (bytes > 0) == (n > 0));
+            EXPECT(gcn_act_grad_workspace_bytes(n, f, &bytes) == GCN_OK && (bytes > 0) == (n > 0));
+            for (int64_t k : {0ll, 5ll, 128ll, 4000ll}) EXPECT(gcn_gemm_epilogue_workspace_bytes(n, f, k, &bytes) == GCN_OK);
+        }
     }
     EXPECT(gcn_rmat_csr_bound(20, 16, GCN_ADD_SELF_LOOPS, &cap, &bytes) == GCN_OK && cap == (33ll << 20));
     EXPECT(gcn_rmat_csr_bound(0, 16, 0, &cap, &bytes) == GCN_ERR_BAD_ARG);
@@ -145,6 +150,30 @@ static void argument_validation() {
     EXPECT(gcn_softmax_xent_f32(-1, 4, nullptr, 4, nullptr, 4, nullptr, 1.0f, nullptr, nullptr, 4, nullptr) != GCN_OK);
     EXPECT(gcn_adam_f32(-1, nullptr, nullptr, nullptr, nullptr, 0.1f, nullptr, 0.9f, 0.999f, 1e-8f, 0.0f, nullptr) != GCN_OK);
     EXPECT(gcn_loss_summary_f32(-1, nullptr, 0, nullptr, 0.0f, nullptr, 0, nullptr, nullptr) != GCN_OK);
+    {   // row norm, 8-bit rows, dense epilogue, distillation
+        int64_t pitch = 0;
+        uint8_t q[64] = {0};
+        int32_t idx[4] = {0};
+        EXPECT(gcn_quant_pitch(100, &pitch) == GCN_OK && pitch == 128);
+        EXPECT(gcn_quant_pitch(0, &pitch) == GCN_ERR_BAD_ARG);
+        EXPECT(gcn_quant_dense_f32(4, 4, nullptr, 16, x, x, 4, nullptr) == GCN_ERR_BAD_ARG);
+        EXPECT(gcn_rms_norm_f32(4, 4, x, 3, nullptr, 0, nullptr, 0.0f, nullptr, 0, x, x, 4, nullptr, 0, nullptr, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_rms_norm_f32(4, 4, x, 4, nullptr, 0, nullptr, -1.0f, nullptr, 0, x, x, 4, nullptr, 0, nullptr, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_rms_norm_f32(4, 4, x, 4, nullptr, 0, nullptr, 0.0f, nullptr, 0, x, x, 4, q, 16, x, nullptr) == GCN_ERR_BAD_ARG);
+        EXPECT(gcn_rms_norm_grad_f32(4, 4, x, 4, x, 4, nullptr, x, nullptr, 0, x, 4, x, nullptr, 0, nullptr) == GCN_ERR_WORKSPACE);
+        EXPECT(gcn_spmm_csr_quant_f32(nullptr, ip, nullptr, nullptr, 4, q, 16, x, x, 4, 0, nullptr, 0, nullptr) == GCN_ERR_BAD_ARG);
+        EXPECT(gcn_gemm_epilogue_f32(4, 4, 4, x, 4, x, 4, 0, nullptr, 9, nullptr, 0, nullptr, 0, x, 4, nullptr, 0, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_gemm_epilogue_f32(4, 4, 4, x, 4, x, 4, 0, nullptr, 0, x, 3, nullptr, 0, x, 4, nullptr, 0, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_act_grad_f32(4, 4, 1, x, 4, nullptr, 4, x, 4, nullptr, nullptr, 0, nullptr) == GCN_ERR_BAD_ARG);
+        EXPECT(gcn_distill_topk_f32(4, 4, x, 4, x, 0, 1, idx, 1, 0, nullptr, 1.0f, 1.0f, nullptr, x, x, 4, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_distill_topk_f32(4, 4, x, 4, x, 0, 1, idx, 1, 1, nullptr, 1.0f, 0.0f, nullptr, x, x, 4, nullptr) ==
+               GCN_ERR_BAD_ARG);
+    }
     // the exchange entry points: every argument check comes before RCCL is opened
     void* comm = nullptr;
     char id[128] = {0};
