@@ -211,7 +211,7 @@ class _QuantDotFn(torch.autograd.Function):
         if grad is not None:
             if ctx.relu:
                 grad = sparse.dropout(grad, 1.0, 0, 0, gate=out)
-            grad = sparse.spmm(ctx.support.transpose(), grad)
+            grad = sparse.spmm(ctx.support.transpose(), grad, own_workspace=True)
         dx, dw = _norm_grads(grad, grad_h, h, weight, inv, ctx.needs_input_grad[2])
         return None, dx, dw, dx if ctx.needs_input_grad[3] else None, None, None
 

@@ -441,14 +441,23 @@ def _two_part_form(a, f, first, b, out):
     return True
 
 
-def spmm(a, b, relu=False, out=None, wide_split=False, out_dropout=None, first=None):
+def _call_workspace(plan, f, device):
+    """(memory, bytes) for the partial rows of one product with ``plan``, freed with the call."""
+    need = ctypes.c_size_t()
+    _lib.call('gcn_spmm_plan_workspace_bytes', plan.handle, f, ctypes.byref(need))
+    return (_workspace(need.value, device) if need.value else None), need.value
+
+
+def spmm(a, b, relu=False, out=None, wide_split=False, out_dropout=None, first=None, own_workspace=False):
     """``a @ b`` for a DeviceCSR ``a`` and dense float32 ``b`` (optionally with ReLU fused).
     ``wide_split`` cuts long rows as a wide product does, whatever the width of ``b``: use it when
     ``b`` is a range of the columns of a wider operand and the bits must match the full product.
     ``out_dropout`` (an OutDropout): the result is written already dropped, after the ReLU.
     ``first``: the operand is ``[first; b]`` -- the rows of ``first`` followed by those of ``b`` (which may be
     None or empty) -- and is read in place, without stacking the two (a stacked copy is made only for
-    layouts the kernels' two-part form does not take)."""
+    layouts the kernels' two-part form does not take).
+    ``own_workspace``: the partial rows of long rows go to memory of this call instead of the plan's, so that products
+    of one plan on several streams, or recorded in several graphs, do not share it."""
     if first is not None:
         _require_cuda(first)
         first = _rowmajor(first)
@@ -471,7 +480,7 @@ def spmm(a, b, relu=False, out=None, wide_split=False, out_dropout=None, first=N
         out = torch.empty((a.n_rows, f), dtype=torch.float32, device=b.device)
     else:
         _check_out(out, a.n_rows, f)
-    ws, ws_bytes = a.plan.workspace(f, b.device)
+    ws, ws_bytes = _call_workspace(a.plan, f, b.device) if own_workspace else a.plan.workspace(f, b.device)
     flags = (_lib.GCN_RELU if relu else 0) | (_lib.GCN_SPLIT_WIDE if wide_split else 0)
     if first is not None:
         d = out_dropout if (out_dropout is not None and out_dropout.keep_prob < 1.0) else None
@@ -1105,12 +1114,9 @@ def spmm_quant(a, q, relu=False, out=None):
             out = q.scales.new_empty((a.n_rows, f))
         else:
             _check_out(out, a.n_rows, f)
-        need, ws = ctypes.c_size_t(), None
-        _lib.call('gcn_spmm_plan_workspace_bytes', a.plan.handle, f, ctypes.byref(need))
-        if need.value:
-            ws = _workspace(need.value, q.data.device)
+        ws, ws_bytes = _call_workspace(a.plan, f, q.data.device)
         _lib.call('gcn_spmm_csr_quant_f32', a.plan.handle, _at(a.indptr), _at(a.indices), _at(a.values), f, _at(q.data), q.ld,
-                  _at(q.scales), _at(out), _ld(out), _lib.GCN_RELU if relu else 0, _at(ws), need.value, _raw_stream())
+                  _at(q.scales), _at(out), _ld(out), _lib.GCN_RELU if relu else 0, _at(ws), ws_bytes, _raw_stream())
     return out
 
 

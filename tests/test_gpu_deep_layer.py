@@ -212,6 +212,41 @@ def test_recording_a_step_while_an_eager_graph_of_its_weights_lives_is_refused()
     assert torch.equal(grad, want)
 
 
+def test_two_recorded_steps_of_one_support_replay_side_by_side():
+    """Hub rows and columns, so that forward and backward products have partial rows: the graphs share no workspace."""
+    import torch
+    from gcn_amd import layers, sparse
+    n = 2500
+    rng = np.random.default_rng(1)
+    hub = np.concatenate([np.zeros(2400, int), np.ones(1500, int)])
+    other = rng.integers(0, n, 3900)
+    rows, cols = np.concatenate([hub, other, rng.integers(0, n, 9000)]), np.concatenate([other, hub, rng.integers(0, n, 9000)])
+    ip, ix, v = sparse.coo_to_csr(n, n, torch.as_tensor(rows).cuda(), torch.as_tensor(cols).cuda(), add_self_loops=True)
+    a = sparse.DeviceCSR(n, n, ip, ix, v.float())
+    assert a.plan.n_chunks > 0 and a.transpose().plan.n_chunks > 0
+    xs = [torch.randn((n, 96), device='cuda', requires_grad=True) for _ in range(2)]
+    up = torch.randn((n, 96), device='cuda')
+
+    def step(x):
+        out = layers.quant_dot(a, x, fuse_relu=True)
+        return out.detach(), torch.autograd.grad(out, x, up)[0]
+    want = [step(x) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for o, w in zip(outs, want) for p, q in zip(o, w))
+
+
 def test_a_plan_of_two_streams():
     import torch
     from gcn_amd import layers

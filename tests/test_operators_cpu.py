@@ -143,3 +143,27 @@ def test_recording_over_a_live_eager_graph_is_refused(monkeypatch):
         assert layers._accumulators(leaf) == []
     del held
     assert len(layers._accumulators(leaf)) == 1
+
+
+def test_calls_go_to_the_device_of_their_tensors(monkeypatch):
+    import torch
+    from gcn_amd import sparse
+
+    class OnGpu(object):
+        def __init__(self, index):
+            self.index, self.device = index, 'cuda:%d' % index
+
+        def get_device(self):
+            return self.index
+    entered = []
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    monkeypatch.setattr(torch.cuda, 'device', lambda index: entered.append(index))
+    assert sparse._on_device(OnGpu(0), None, OnGpu(0)) is sparse._NO_GUARD and entered == []
+    sparse._on_device(OnGpu(1), OnGpu(1))
+    assert entered == [1]
+    with pytest.raises(ValueError):
+        sparse._on_device(OnGpu(0), OnGpu(1))
+    with pytest.raises(ValueError):
+        sparse._on_device(OnGpu(0), torch.ones(1))
+    with pytest.raises(ValueError):
+        sparse._on_device(torch.ones(1))
