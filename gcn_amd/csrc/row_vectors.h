@@ -45,9 +45,9 @@ __device__ __forceinline__ void load_row(const float* __restrict__ row, int sub,
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
         // a vector that begins in the row may end in the next one, whose values are replaced below; behind the last
-        // row there may be nothing
+        // row there may be nothing, and rows of one column may end less than a vector behind this one
         const int at = 4 * (sub + G * v);
-        if (!last || at + 4 <= f) {
+        if ((!last && f >= 2) || at + 4 <= f) {
             const f4u t = *reinterpret_cast<const f4u*>(row + (at < f ? at : 0));
             x[v][0] = t.x;
             x[v][1] = t.y;
