@@ -22,6 +22,7 @@
 namespace gcn {
 
 constexpr int kDistillMaxK = 256;
+constexpr int kWaveRowC = 1024;          // wider rows belong to a workgroup each
 
 struct DistillArgs {
     int64_t n;                // rows of this launch
@@ -526,7 +527,7 @@ static void launch_distill(const DistillArgs& a, hipStream_t st) {
     else if (a.c <= 128) launch_group<16, 2>(a, st);
     else if (a.c <= 256) launch_group<32, 2>(a, st);
     else if (a.c <= 512) launch_row<64, 2, 256>(a, st);
-    else if (a.c <= 1024) launch_row<64, 4, 256>(a, st);
+    else if (a.c <= kWaveRowC) launch_row<64, 4, 256>(a, st);
     else if (a.c <= 4096) launch_row<256, 4, 256>(a, st);
     else if (a.c <= 8192) launch_row<256, 8, 256>(a, st);
     else if (a.c <= 16384) launch_row<1024, 4, 1024>(a, st);
@@ -557,11 +558,11 @@ int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx,
     if (!logits || !values || !indices) return fail(GCN_ERR_BAD_ARG, "null pointer");
     if (row_stats && ((uintptr_t)row_stats & 7)) return fail(GCN_ERR_BAD_ARG, "row_stats must be 8-byte aligned");
     if (!row_stats && !dlogits) return GCN_OK;
-    // a launch counts its threads in 32 bits: 2^22 - 1 rows of up to 1024 threads at a time
-    constexpr int64_t kSlice = ((int64_t)1 << 22) - 1;
+    // a launch counts its threads in 32 bits: rows of at most 64 threads, or of up to 1024
+    const int64_t slice = (c <= kWaveRowC ? (int64_t)1 << 26 : (int64_t)1 << 22) - 4;
     const int64_t value_size = value_type == GCN_F32 ? 4 : 2;
-    for (int64_t r = 0; r < n; r += kSlice) {
-        const DistillArgs a = {std::min(kSlice, n - r), 1.0f / (float)n, (int)c, logits + r * ldx, ldx,
+    for (int64_t r = 0; r < n; r += slice) {
+        const DistillArgs a = {std::min(slice, n - r), 1.0f / (float)n, (int)c, logits + r * ldx, ldx,
                                (const char*)values + r * ldv * value_size, value_type, ldv, indices + r * ldi, ldi, (int)k,
                                mask ? mask + r : nullptr, 1.0f / mask_mean, temperature, 1.4426950408889634f / temperature,
                                row_stats ? row_stats + 2 * r : nullptr, dlogits ? dlogits + r * ldd : nullptr, ldd, upstream};

@@ -187,19 +187,20 @@ def test_views_streams_and_a_replayed_graph():
         assert torch.equal(s, stats) and torch.equal(g, grad) and torch.equal(sparse.loss_summary(s, None, 0.0), summary)
 
 
-def test_more_rows_than_one_launch_takes_and_offsets_past_32_bits():
-    """4.3 million rows of 601 classes: 10 GB of logits, two slices, element offsets past 2^31; sampled rows against the
-    formula."""
+@pytest.mark.parametrize('n,c,at', [(4300001, 601, 3573000), (67109001, 9, (1 << 26) - 4), (4194400, 1030, (1 << 22) - 4)])
+def test_more_rows_than_one_launch_takes_and_offsets_past_32_bits(n, c, at):
+    """Element offsets past 2^31, and more rows than one launch takes of narrow and of wide ones; sampled rows against the
+    formula, among them those around `at`: where the element offset passes 2^31, or where the second launch begins."""
     import torch
     from gcn_amd import sparse
-    n, c, k = 4300001, 601, 3
+    k = 3
     if torch.cuda.mem_get_info()[0] < 40 << 30:
         pytest.skip('needs 40 GB of free device memory')
     logits = torch.empty((n, c), device='cuda').normal_(generator=torch.Generator('cuda').manual_seed(3))
     values = torch.randn((n, k), device='cuda')
     idx = torch.randint(0, c, (n, k), device='cuda', dtype=torch.int32)
     stats, grad = sparse.distill_topk(logits, values, idx, None, 1.0)
-    for lo in (0, 3573000, 4194290, n - 40):
+    for lo in (0, at - 20, 4194290, n - 40):
         rows = slice(lo, lo + 40)
         ref = list(_reference(logits[rows], values[rows], idx[rows], None, 1.0, 1.0))
         ref[2], ref[3] = ref[2] * 40 / n, ref[3] * 40 / n
