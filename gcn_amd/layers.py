@@ -145,25 +145,44 @@ class _GatedGemmFn(torch.autograd.Function):
         return d_h, d_w, None
 
 
+# nodes whose own inputs have been through _accumulators
+_MARKED_BELOW = frozenset(('_RmsNormFnBackward', '_QuantDotFnBackward', '_DenseFnBackward'))
+
+
 def _accumulators(*inputs):
     """The gradient accumulators of the leaves among the inputs, to be held over the call that uses them.  Refuses to record
-    a differentiable call while an eager graph over the same leaves lives: such a graph keeps the accumulators, which
-    belong to the stream it was built on, and a backward pass recorded over them waits for
-    that stream, which ends the capture and the process.  Eager calls mark the accumulators; a mark dies with the
-    accumulator, that is, with the last eager graph over the leaf."""
+    a differentiable call while an eager graph over the same leaves lives, those reached through other operations (a
+    transposed weight) among them: such a graph keeps the accumulators, which belong to the stream it was built on, and a
+    backward pass recorded over them waits for that stream, which ends the capture and the process.  Eager calls
+    mark the nodes their inputs hang on; a mark dies with its node, that is, with the last eager graph that holds it."""
     held = []
     if not torch.is_grad_enabled():
         return held
-    capturing = torch.cuda.is_current_stream_capturing()
+    capturing, below = torch.cuda.is_current_stream_capturing(), []
     for t in inputs:
-        if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf:
-            node = torch.autograd.graph.get_gradient_edge(t).node
-            if not capturing:
-                node.metadata['gcn_amd_eager'] = True
-            elif node.metadata.get('gcn_amd_eager'):
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            node = t.grad_fn
+            if node is None:
+                node = torch.autograd.graph.get_gradient_edge(t).node
+                held.append(node)
+            below.append(node)
+    seen = set()
+    while below:
+        node = below.pop()
+        if capturing:
+            if node.metadata.get('gcn_amd_eager'):
                 raise RuntimeError('an eager autograd graph over an input of this recorded call is alive: drop its outputs '
                                    'and losses before capturing')
-            held.append(node)
+            if node in seen:
+                continue
+            seen.add(node)
+        else:
+            if node.metadata.get('gcn_amd_eager'):
+                continue
+            node.metadata['gcn_amd_eager'] = True
+            if type(node).__name__ in _MARKED_BELOW:
+                continue
+        below.extend(n for n, _ in node.next_functions if n is not None)
     return held
 
 

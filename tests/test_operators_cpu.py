@@ -145,6 +145,26 @@ def test_recording_over_a_live_eager_graph_is_refused(monkeypatch):
     assert len(layers._accumulators(leaf)) == 1
 
 
+def test_recording_over_an_eager_graph_of_a_transposed_leaf_is_refused(monkeypatch):
+    import torch
+    from gcn_amd import layers
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: capturing[0])
+    w, x = torch.ones((2, 3), requires_grad=True), torch.ones((3, 2), requires_grad=True)
+    turned = w.t() * 2
+    moved = x + w.sum()
+    assert layers._accumulators(turned, moved) == []
+    loss = (turned * moved).sum()               # what a wrapper's call does with them
+    capturing[0] = True
+    for again in (w, x, w.t(), turned, moved.exp(), (w.t() + 1).exp()):
+        with pytest.raises(RuntimeError):
+            layers._accumulators(again)
+    other = torch.ones(3, requires_grad=True)
+    assert len(layers._accumulators(other, other * 2)) == 1
+    del turned, moved, loss, again
+    assert len(layers._accumulators(w, w.t().exp(), x)) == 2
+
+
 def test_calls_go_to_the_device_of_their_tensors(monkeypatch):
     import torch
     from gcn_amd import sparse
