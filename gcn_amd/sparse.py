@@ -443,9 +443,11 @@ def _two_part_form(a, f, first, b, out):
 
 def _call_workspace(plan, f, device):
     """(memory, bytes) for the partial rows of one product with ``plan``, freed with the call."""
+    if plan.n_chunks == 0:
+        return None, 0
     need = ctypes.c_size_t()
     _lib.call('gcn_spmm_plan_workspace_bytes', plan.handle, f, ctypes.byref(need))
-    return (_workspace(need.value, device) if need.value else None), need.value
+    return _workspace(need.value, device), need.value
 
 
 def spmm(a, b, relu=False, out=None, wide_split=False, out_dropout=None, first=None, own_workspace=False):
