@@ -13,7 +13,8 @@
 // instruction of a group reads 16 G consecutive bytes.  Sums, the maximum and the weight's gradient are float32.
 // Measured, compulsory bytes over time (a large copy: 4.7 TB/s), rows of 1 GB: 8-bit output with residual 4.8 to 5.2 TB/s at
 // 16, 64, 256, 500, 1433, 2048 and 8192 columns (100: 4.0, whose 112 of 128 bytes a row are partial lines), float32 output
-// 4.9 to 5.3, gradients 4.3 to 5.0; past 16,384 columns the registers of a row no longer fit and the gradient falls to 1.4.
+// 4.9 to 5.3, gradients 4.3 to 5.0; past 16,384 columns 3.6 to 4.4 forward, and the gradient, which reads its rows twice there,
+// 2.5 to 3.2 (1.4 with the rows held in registers, which then spill).
 // A wave a row at 1433 columns (eight vectors a lane, two waves a SIMD) ran the gradient at 2.6 instead of 4.7.
 #include <algorithm>
 
@@ -238,6 +239,75 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_grad_kernel(NormGradArgs a, in
     }
 }
 
+// Rows past 16,384 columns, a workgroup a row: two of its operands and the weight's gradient do not fit the 128 registers of
+// a lane among 1024 (the kernel above spilled 338 of them).  The weight's gradient stays in LDS, every lane at its own
+// columns, and the row is read a second time, from the caches, for dx.
+__global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(NormGradArgs a, int tile) {
+    constexpr int G = 1024, kDepth = 4;
+    __shared__ float lds[2][16];
+    __shared__ __attribute__((aligned(16))) float dw[kNormMaxF];
+    const int sub = threadIdx.x, f = a.f;
+    const float inv_f = 1.0f / (float)f;
+    for (int c = 4 * sub; c < f; c += 4 * G) *reinterpret_cast<float4*>(dw + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // calls use(column, g, h) for the lane's vectors of a row, kDepth of them in flight; g = dy without the weight
+    auto walk = [&](const float* dy, const float* h, auto use) {
+        for (int c0 = 4 * sub; c0 < f; c0 += 4 * G * kDepth) {
+            float g[kDepth][4], x[kDepth][4], w[kDepth][4];
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) {
+                const int c = c0 + 4 * G * u < f ? c0 + 4 * G * u : 4 * sub;
+                load_cols(dy, c, f, g[u]);
+                load_cols(h, c, f, x[u]);
+                if (a.w) {
+                    load_cols(a.w, c, f, w[u]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[u][e] = 1.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u)
+                if (c0 + 4 * G * u < f) use(c0 + 4 * G * u, g[u], x[u], w[u]);
+        }
+    };
+    for (int t = 0; t < tile; ++t) {
+        const int64_t i = (int64_t)blockIdx.x * tile + t;
+        if (i >= a.n) break;                                                  // uniform in the workgroup
+        const float *dy = a.dy + i * a.lddy, *h = a.h + i * a.ldh;
+        const float inv = a.inv[i];
+        float along = 0.0f;
+        walk(dy, h, [&](int c, const float (&g)[4], const float (&x)[4], const float (&w)[4]) {
+            float4 s = *reinterpret_cast<float4*>(dw + c);
+            s.x = fmaf(g[0], x[0] * inv, s.x);
+            s.y = fmaf(g[1], x[1] * inv, s.y);
+            s.z = fmaf(g[2], x[2] * inv, s.z);
+            s.w = fmaf(g[3], x[3] * inv, s.w);
+            *reinterpret_cast<float4*>(dw + c) = s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) along = fmaf(g[e] * w[e], x[e], along);
+        });
+        if (!a.dx) continue;
+        along = row_reduce<G, false>(along, lds[t & 1]);
+        const float back = along * inv_f * inv * inv;
+        walk(dy, h, [&](int c, const float (&g)[4], const float (&x)[4], const float (&w)[4]) {
+            float u[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4];
+            if (a.dh) load_cols(a.dh + i * a.lddh, c, f, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] = inv * (g[e] * w[e] - x[e] * back);
+                if (a.dh) o[e] += u[e];
+            }
+            store_cols(a.dx + i * a.lddx, c, f, o);
+        });
+    }
+    if (!a.part) return;
+    for (int c = 4 * sub; c < f; c += 4 * G) {
+        const float4 s = *reinterpret_cast<const float4*>(dw + c);
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        store_cols(a.part + (int64_t)blockIdx.x * f, c, f, v);
+    }
+}
+
 // out[c] = sum over the rows of part [rows x f]: 16 columns a workgroup, 64 strided sums a column, eight of their rows in
 // flight, added pairwise in a fixed tree.  (64 columns a workgroup and one row in flight: 38 us for 1974 x 256, 50 us for
 // 1924 x 1433; this form: 7 and 9 us.)
@@ -293,8 +363,7 @@ static inline int norm_rows(int64_t f) {
     else if (f <= 2048) { LAUNCH(256, 2, 256); } \
     else if (f <= 4096) { LAUNCH(256, 4, 256); } \
     else if (f <= 8192) { LAUNCH(256, 8, 256); } \
-    else if (f <= 16384) { LAUNCH(1024, 4, 1024); } \
-    else { LAUNCH(1024, 8, 1024); }
+    else if (f <= 16384) { LAUNCH(1024, 4, 1024); }
 
 // row groups a workgroup walks one after the other: one until there are workgroups for every compute unit's slots
 static inline int norm_tile(int64_t n, int64_t f) {
@@ -351,6 +420,7 @@ int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const fl
 #define GCN_LAUNCH_NORM(G, VPL, BLOCK) \
     rms_norm_kernel<G, VPL, BLOCK><<<(unsigned)blocks, BLOCK, 0, (hipStream_t)stream>>>(a, tile)
     GCN_NORM_BY_WIDTH(GCN_LAUNCH_NORM)
+    else { GCN_LAUNCH_NORM(1024, 8, 1024); }
 #undef GCN_LAUNCH_NORM
     GCN_LAUNCH_CHECK();
     return GCN_OK;
@@ -384,6 +454,7 @@ int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, c
 #define GCN_LAUNCH_NORM(G, VPL, BLOCK) \
     rms_norm_grad_kernel<G, VPL, BLOCK><<<(unsigned)blocks, BLOCK, 0, st>>>(a, tile)
     GCN_NORM_BY_WIDTH(GCN_LAUNCH_NORM)
+    else rms_norm_grad_wide_kernel<<<(unsigned)blocks, 1024, 0, st>>>(a, tile);
 #undef GCN_LAUNCH_NORM
     GCN_LAUNCH_CHECK();
     return dweight ? launch_column_sums(blocks, f, (const float*)workspace, dweight, st) : GCN_OK;

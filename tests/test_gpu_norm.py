@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 SHAPES = [(1, 1), (1, 7), (3, 2), (5, 3), (2708, 16), (130, 17), (77, 31), (65, 33), (9, 63), (1000, 64), (33, 100),
           (19, 127), (5, 129), (515, 256), (7, 257), (64, 500), (3, 511), (6, 1000), (11, 1433), (4, 2047), (3, 2049),
-          (5, 3703), (2, 4097), (2, 8191), (2, 8193), (1, 16383), (2, 20001), (1, 32768)]
+          (5, 3703), (2, 4097), (2, 8191), (2, 8193), (1, 16383), (2, 20001), (1, 32768),
+          (5000, 16387)]
 
 
 def _inputs(n, f, seed=0):
@@ -115,7 +116,7 @@ def test_gradient_against_differences():
         assert abs(slope - float(dw[j])) <= 1e-5
 
 
-@pytest.mark.parametrize('f', [16, 37, 256, 2500])
+@pytest.mark.parametrize('f', [16, 37, 256, 2500, 17003])
 def test_views_outputs_and_aliases(f):
     """Rows inside a wider matrix at an odd offset, outputs given by the caller, h written over x or the residual,
     the memory between and behind the rows untouched."""
