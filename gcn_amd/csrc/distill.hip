@@ -8,10 +8,10 @@
 // Bound by memory: the logits are read once and their gradient is written once, the exponentials of a row staying in
 // registers between the two; rows outside the mask are not read at all.  Rows of up to 256 classes belong to G lanes with
 // four or eight classes each, so that a wave holds 64 / G rows and the reductions a row needs are shared by them; wider
-// ones to a wave or a workgroup, up to 65,536 classes; beyond that the row is read a second time for its gradient.
+// ones to a wave or a workgroup, up to 32,768 classes; beyond that the row is read a second time for its gradient.
 // Measured, compulsory bytes over time (a large copy: 4.7 TB/s): 4 M x 47 classes, 5 listed: 390 us, 4.5 TB/s;
 // 4 M x 7, 3 listed: 90 us, 4.0; 1 M x 200, 20 listed: 389 us, 4.7; 8,192 x 32,768, 32 listed: 416 us, 5.2;
-// 2,048 x 65,536: 426 us, 2.5 (one workgroup a compute unit, and it spills).
+// read twice, 2,048 x 65,536: 292 us, 3.7 (held in registers, which then spill, 426 us); 8,192 x 32,768 read twice: 497 us.
 #include <algorithm>
 #include <hip/hip_fp16.h>
 
@@ -435,7 +435,21 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     if (lister) listed_grad(a, i, lane, list, xm, qs, pscale, scale);
 }
 
-// any number of classes: the row is read twice, the second time for its gradient
+// Calls use(column, values) for the lane's vectors of a row of any length, kDepth of them in flight.
+template <int G, class F>
+__device__ __forceinline__ void walk_row(const float* __restrict__ row, int sub, int c, F use) {
+    constexpr int kDepth = 4;
+    for (int64_t c0 = 4 * sub; c0 < c; c0 += 4 * G * kDepth) {
+        float v[kDepth][4];
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) load_cols(row, c0 + 4 * G * u < c ? (int)c0 + 4 * G * u : 4 * sub, c, v[u]);
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u)
+            if (c0 + 4 * G * u < c) use((int)c0 + 4 * G * u, v[u]);
+    }
+}
+
+// any number of classes: the row is read twice, the second time, from the caches, for its gradient
 __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     constexpr int G = 1024;
     __shared__ float lds[3][16];
@@ -449,7 +463,10 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     float* gr = a.grad ? a.grad + i * a.ldg : nullptr;
     if (m == 0) {
         if (gr)
-            for (int64_t c = tid; c < a.c; c += G) gr[c] = 0.0f;
+            for (int64_t c = 4 * tid; c < a.c; c += 4 * G) {
+                const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                store_cols(gr, (int)c, a.c, zero);
+            }
         if (a.stats && tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * i) = make_float2(0.0f, 0.0f);
         return;
     }
@@ -460,15 +477,24 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     // running maximum and the sum relative to it, per lane; NaN ends up in the sum
     float run = -INFINITY, s = 0.0f;
     int first = 0x7fffffff;
-    for (int64_t c = tid; c < a.c; c += G) {
-        const float v = xr[c];
-        if (v > run) {
-            s *= __builtin_amdgcn_exp2f((run - v) * a.to_log2);
-            run = v;
-            first = (int)c;
+    walk_row<G>(xr, tid, a.c, [&](int c, const float (&v)[4]) {
+        float most = -INFINITY;
+        int at = 0;
+#pragma unroll
+        for (int e = 3; e >= 0; --e)
+            if (c + e < a.c && v[e] >= most) {
+                most = v[e];
+                at = c + e;
+            }
+        if (most > run) {
+            s *= __builtin_amdgcn_exp2f((run - most) * a.to_log2);
+            run = most;
+            first = at;
         }
-        s += v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v - run) * a.to_log2);
-    }
+        const float ref = run > -INFINITY ? run : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += c + e < a.c ? __builtin_amdgcn_exp2f((v[e] - ref) * a.to_log2) : 0.0f;
+    });
     const float xm = wide_reduce<G, OpMax>(run, lds[0]);
     const Listed l = shared_list;
     if (run != xm) first = 0x7fffffff;
@@ -479,7 +505,12 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(DistillArgs a) {
     const float scale = l.tsum == l.tsum ? w * (a.upstream ? *a.upstream : 1.0f) * a.t * a.per_row : NAN;
     const float qs = 1.0f / s;
     if (gr)
-        for (int64_t c = tid; c < a.c; c += G) gr[c] = l.any ? __builtin_amdgcn_exp2f((xr[c] - xm) * a.to_log2) * (qs * scale) : 0.0f;
+        walk_row<G>(xr, tid, a.c, [&](int c, const float (&v)[4]) {
+            float g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = l.any ? __builtin_amdgcn_exp2f((v[e] - xm) * a.to_log2) * (qs * scale) : 0.0f;
+            store_cols(gr, c, a.c, g);
+        });
     if (a.stats) {
         first = __float_as_int(wide_reduce<G, OpMinInt>(__int_as_float(first), lds[2]));
         if (tid < 64) {
@@ -532,7 +563,6 @@ static void launch_distill(const DistillArgs& a, hipStream_t st) {
     else if (a.c <= 8192) launch_row<256, 8, 256>(a, st);
     else if (a.c <= 16384) launch_row<1024, 4, 1024>(a, st);
     else if (a.c <= 32768) launch_row<1024, 8, 1024>(a, st);
-    else if (a.c <= 65536) launch_row<1024, 16, 1024>(a, st);
     else distill_long_kernel<<<(unsigned)a.n, 1024, 0, st>>>(a);
 }
 

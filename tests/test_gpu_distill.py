@@ -65,7 +65,8 @@ def _check(stats, grad, ref):
 SHAPES = [(1, 1, 1), (5, 2, 2), (1, 3, 5), (2708, 7, 3), (333, 4, 4), (130, 6, 1), (129, 8, 8), (77, 9, 4), (1000, 16, 5),
           (515, 17, 20), (64, 33, 7), (4099, 47, 5), (31, 64, 64), (9, 65, 3), (21, 128, 128), (7, 130, 256), (33, 256, 9),
           (5, 257, 65), (6, 512, 32), (3, 513, 100), (5, 1000, 256), (2, 1025, 7), (3, 4097, 33), (2, 8193, 64),
-          (2, 20000, 200), (1, 32768, 32), (1, 50001, 5), (1, 65536, 256), (2, 65537, 17), (1, 200003, 50)]
+          (2, 20000, 200), (1, 32768, 32), (1, 50001, 5), (1, 65536, 256), (2, 65537, 17), (1, 200003, 50),
+          (300, 33333, 9)]
 
 
 @pytest.mark.parametrize('n,c,k', SHAPES)
