@@ -376,6 +376,22 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             rb[p] = make_float4(t[0], t[1], t[2], t[3]);
         }
     };
+    // A tile that n cuts, a whole stage of k that is not B's [k x n] last row's: what columns past n give is not stored, so
+    // they repeat a column of the matrix, and a vector that n cuts ends in the next row.
+    auto load_b_edge = [&](int64_t k0) {
+#pragma unroll
+        for (int p = 0; p < kBPer; ++p) {
+            const int u = tid + kBlock * p;
+            if (!kBAll && u >= kBUnits) continue;
+            if (TRANS_B) {
+                const int64_t gc = n0 + u / kKQ < n ? n0 + u / kKQ : n - 1;
+                rb[p] = load_quad(b + gc * ldb + k0 + (u % kKQ) * 4);
+            } else {
+                const int64_t gc = n0 + (u % (BN / 4)) * 4;
+                rb[p] = load_quad(b + (k0 + u / (BN / 4)) * ldb + (gc < n ? gc : n0));
+            }
+        }
+    };
     auto store_tile = [&]() {
 #pragma unroll
         for (int i = 0; i < kAPer; ++i) *reinterpret_cast<float4*>(as + (a_r + kARows * i) * kAPitch + a_kq) = ra[i];
@@ -440,6 +456,7 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
     const bool b_inside = n0 + BN <= n;
     const bool interior = (m0 + kBM <= m) && (n0 + BN <= n);
     const int64_t n_full = a_inside ? k / kBK : 0;       // leading k tiles whose A loads need no guards
+    const int64_t n_edge = TRANS_B ? n_full : ldb < 4 ? 0 : n_full * kBK < k ? n_full : n_full - 1;   // those load_b_edge takes
     if (n_ktiles > 0) {
         if (n_full > 0)
             load_a_fast(0);
@@ -447,6 +464,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             load_a_guarded(0);
         if (n_full > 0 && b_inside)
             load_b_fast(0);
+        else if (n_edge > 0)
+            load_b_edge(0);
         else
             load_b_guarded(0);
         store_tile();
@@ -463,9 +482,11 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             __syncthreads();
         }
     } else {
-        for (; t + 1 < n_full; ++t) {  // edge tile in n (a narrow output): only the small B tile is guarded
+        // edge tile in n (a narrow output).  With load_b_guarded in load_b_edge's place: 1M x 256 x 47 455 us against 400,
+        // 652,304 x 902 x 17 685 against 610
+        for (; t + 1 < n_edge; ++t) {
             load_a_fast((t + 1) * kBK);
-            load_b_guarded((t + 1) * kBK);
+            load_b_edge((t + 1) * kBK);
             compute();
             __syncthreads();
             store_tile();
@@ -652,11 +673,18 @@ __device__ __forceinline__ uint32_t quad_read(uint32_t x, int src) {
     }
 }
 
+// The stages of k that the ragged kernel loads in vectors of four: all whole ones, but not B's [k x n] last row where a
+// vector of it could pass its end.
+__host__ __device__ constexpr int ragged_stages(int64_t n, int64_t k, bool trans_b) {
+    return (int)((trans_b || n % 4 == 0 ? k : k - 1) / 32);
+}
+
 // RAGGED (EPI == kEpiLayer): any m, n and k and any alignment.  Rows of A past the end (and columns of B past n) repeat
-// the last one -- what they give is not stored --, and the last 1 to 32 of k, loaded element by element with zeros
-// past the end, come after n_ktiles whole stages: every address lies inside the operands, and the main loop has no test.
-// The guarded kernel ran 150,001 x 500 x 256 at 103 TFLOP/s, this one at 109, and its gradient
-// 150,001 x 256 x 500 (B [n x k]) at 113 instead of 97.  Same order of additions.
+// the last one -- what they give is not stored --, and the last of k, loaded element by element with zeros past the
+// end, come after n_ktiles whole stages (ragged_stages): every address lies inside the operands, and the main loop has no test.
+// The guarded kernel ran 150,001 x 500 x 256 at 100 TFLOP/s, this one at 113, and its gradient
+// 150,001 x 256 x 500 (B [n x k]) at 114 instead of 97.  Same order of additions.  (With the last stage as a branch of
+// the loop and the first one peeled the kernel took 168 registers, three waves a SIMD instead of four: 109 TFLOP/s.)
 template <bool TRANS_B, int EPI, bool A_MASK = false, bool RAGGED = false>
 __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int n_ktiles,
                                                                const float* __restrict__ a, int64_t lda,
@@ -671,7 +699,7 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
         b += TRANS_B ? (int64_t)from : (int64_t)from * ldb;
         c += (int64_t)blockIdx.z * m * n;
         k = min(k - from, k_cut);
-        n_ktiles = (k - 1) / 32;
+        n_ktiles = ragged_stages(n, k, TRANS_B);
     }
     constexpr int kBM = 128, BN = 128, kBK = 32, MT = 2, NT = 2;
     constexpr int kAPitch = kBK + 4, kBPitch = BN + 4;
@@ -849,21 +877,27 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_panels_kernel(int tiles_m, int
         load_stage(0, 0);
     store_tile();
     __syncthreads();
-    if (RAGGED && n_ktiles == 0) {
-        compute(std::true_type{});
-    } else if (RAGGED) {
+    if (RAGGED) {
+        // the accumulators start as zeros here: one copy of the loop's body less
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
         int a_k = 0, b_k = 0;
-        for (int t = 1; t <= n_ktiles; ++t) {
+        for (int t = 1; t < n_ktiles; ++t) {
             a_k += kBK * 4;
             b_k += b_kstep;
-            if (t < n_ktiles)
-                load_stage(a_k, b_k);
-            else
-                load_tail(t * kBK);
-            if (t == 1)
-                compute(std::true_type{});
-            else
-                compute(std::false_type{});
+            load_stage(a_k, b_k);
+            compute(std::false_type{});
+            __syncthreads();
+            store_tile();
+            __syncthreads();
+        }
+        if (n_ktiles > 0 && n_ktiles * kBK < k) {
+            load_tail(n_ktiles * kBK);
+            compute(std::false_type{});
             __syncthreads();
             store_tile();
             __syncthreads();
@@ -1115,7 +1149,7 @@ static int launch_gemm(int64_t m, int64_t n, int64_t k, const float* a, int64_t 
         const dim3 grid((unsigned)(8 * col_tiles), (unsigned)ceil_div(panels, (int64_t)8));
 #define GCN_RAGGED_GO(TB)                                                                                           \
     gemm_panels_kernel<TB, kEpiLayer, false, true><<<grid, kBlock, 0, st>>>(                                        \
-        (int)panels, (int)((k - 1) / 32), a, lda, b, ldb, c, ldc, 0, nullptr, 0, 1.0f, kNoInMask, no_drop, col_tiles >= 16, ep, m, \
+        (int)panels, ragged_stages(n, k, trans_b), a, lda, b, ldb, c, ldc, 0, nullptr, 0, 1.0f, kNoInMask, no_drop, col_tiles >= 16, ep, m, \
         n, (int)k, 0)
         if (trans_b)
             GCN_RAGGED_GO(true);
@@ -1682,10 +1716,11 @@ int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64
             return rc;
         return launch_join_splits(m, n, cuts, (const float*)workspace, ep, c, ldc, st);
     }
-    // fewer than four 128-column tiles a compute unit: tiles half as wide balance better (20,000 x 512 x 512 168 -> 129 us;
-    // 71,428 x 208 x 355, 1674 tiles, keeps the wide ones: 158 against 167)
+    // tiles of 64 columns balance better where there are fewer than four of 128 a compute unit (20,000 x 512 x 512 168 -> 129 us;
+    // 71,428 x 208 x 355, 1674 tiles, keeps the wide ones: 121 against 167), and pad less where n wants an odd number of
+    // them (100,000 x 300 x 192 151 -> 134 us, x 448 284 -> 274; nothing left to gain at 576)
     if (n <= 32) return launch_gemm<128, 32>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
-    if (n <= 64 || layer_tiles(m, n) < 1024) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
+    if (n <= 64 || layer_tiles(m, n) < 1024 || (n < 512 && ceil_div(n, (int64_t)64) % 2)) return launch_gemm<128, 64>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
     return launch_gemm<128, 128>(m, n, k, a, lda, b, ldb, trans_b, c, ldc, 0, st, nullptr, 0, 1.0f, nullptr, nullptr, &ep);
 }
 

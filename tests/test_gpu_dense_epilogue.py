@@ -198,3 +198,22 @@ def test_empty_and_refusals():
                  lambda: sparse.act_grad(g.cpu(), r, 'relu')):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize('trans_b', [False, True])
+@pytest.mark.parametrize('m,n,k', [(300, 17, 96), (300, 47, 70), (257, 134, 64), (300, 200, 96), (1500, 16, 1433), (150000, 130, 64),
+                                   (150001, 200, 65), (129, 3, 33), (129, 1, 64), (5000, 333, 300)])
+def test_operands_inside_matrices_of_nan(m, n, k, trans_b):
+    """What lies around the operands does not reach the result, and the result has the bits of the packed operands'."""
+    import torch
+    from gcn_amd import sparse
+    a = torch.randn((m, k), device='cuda')
+    b = torch.randn((n, k) if trans_b else (k, n), device='cuda')
+    room_a = torch.full((m + 2, k + 5), float('nan'), device='cuda')
+    room_b = torch.full((b.shape[0] + 2, b.shape[1] + 7), float('nan'), device='cuda')
+    room_a[1:m + 1, 2:2 + k] = a
+    room_b[1:b.shape[0] + 1, 3:3 + b.shape[1]] = b
+    va, vb = room_a[1:m + 1, 2:2 + k], room_b[1:b.shape[0] + 1, 3:3 + b.shape[1]]
+    for f in (lambda x, y: sparse.gemm_epilogue(x, y, trans_b=trans_b, act='silu'), lambda x, y: sparse.gemm(x, y, trans_b=trans_b),
+              lambda x, y: sparse.gemm(x, y, trans_b=trans_b, relu=True)):
+        assert torch.equal(f(va, vb), f(a, b))
