@@ -168,6 +168,10 @@ static void argument_validation() {
                GCN_ERR_BAD_ARG);
         EXPECT(gcn_gemm_epilogue_f32(4, 4, 4, x, 4, x, 4, 0, nullptr, 0, x, 3, nullptr, 0, x, 4, nullptr, 0, nullptr) ==
                GCN_ERR_BAD_ARG);
+        EXPECT(gcn_gemm_epilogue_f32(4, 4, 4, x, 4, x, 4, 0, nullptr, 0, nullptr, 0, nullptr, 0, x, 4, nullptr, 0, nullptr) ==
+               GCN_ERR_BAD_ARG);
+        EXPECT(gcn_distill_topk_f32(4, 4, x, 4, x, 0, 1, idx, 1, 1, nullptr, 1.0f, 1.0f, nullptr, nullptr, x, 4, nullptr) ==
+               GCN_ERR_BAD_ARG);
         EXPECT(gcn_act_grad_f32(4, 4, 1, x, 4, nullptr, 4, x, 4, nullptr, nullptr, 0, nullptr) == GCN_ERR_BAD_ARG);
         EXPECT(gcn_distill_topk_f32(4, 4, x, 4, x, 0, 1, idx, 1, 0, nullptr, 1.0f, 1.0f, nullptr, x, x, 4, nullptr) ==
                GCN_ERR_BAD_ARG);

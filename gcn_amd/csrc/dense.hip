@@ -1706,10 +1706,11 @@ int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64
     hipStream_t st = (hipStream_t)stream;
     const EpiArgs ep = {bias, residual, residual ? ldr : 0, pre, pre ? ldp : 0, act};
     const int64_t cuts = layer_cuts(m, n, k);
+    const size_t need = cuts > 1 ? (size_t)cuts * (size_t)m * (size_t)n * sizeof(float) : 0;
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
+    if (c && (c == a || c == b || c == pre)) return fail(GCN_ERR_BAD_ARG, "the result needs memory of its own");
     if (cuts > 1) {
-        const size_t need = (size_t)cuts * (size_t)m * (size_t)n * sizeof(float);
-        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
-            return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
         if (int rc = n <= 32   ? launch_cuts<32>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)
                      : n <= 64 ? launch_cuts<64>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)
                                : launch_cuts<128>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st))

@@ -586,6 +586,7 @@ int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx,
     if (!(temperature > 0.0f) || !(temperature < INFINITY)) return fail(GCN_ERR_BAD_ARG, "the temperature must be positive");
     if (n == 0) return GCN_OK;
     if (!logits || !values || !indices) return fail(GCN_ERR_BAD_ARG, "null pointer");
+    if (dlogits == logits) return fail(GCN_ERR_BAD_ARG, "the gradient needs memory of its own: the logits are read after its first stores");
     if (row_stats && ((uintptr_t)row_stats & 7)) return fail(GCN_ERR_BAD_ARG, "row_stats must be 8-byte aligned");
     if (!row_stats && !dlogits) return GCN_OK;
     // a launch counts its threads in 32 bits: rows of at most 64 threads, or of up to 1024

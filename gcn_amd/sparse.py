@@ -1137,7 +1137,7 @@ def _act_code(act):
 
 def gemm_epilogue(a, b, trans_b=False, bias=None, act=None, residual=None, out=None, want_pre=False):
     """``act(a @ b + bias) + residual`` (``a @ b.T`` with ``trans_b``) in one product; ``act``: None, 'relu', 'gelu' (the
-    normal distribution function, no tanh) or 'silu'.  ``residual`` may be ``out`` itself.  With ``want_pre`` returns
+    normal distribution function, no tanh) or 'silu'.  ``residual`` may be ``out`` itself, ``a`` and ``b`` not.  With ``want_pre`` returns
     ``(result, pre)``, ``pre = a @ b + bias`` as ``act_grad`` wants it."""
     code = _act_code(act)
     with _on_device(a, b, bias, residual, out):

@@ -573,7 +573,7 @@ int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, con
  * epilogue in its store.  bias [n], residual [m x n] (may be C itself) and pre may be NULL; pre [m x n] receives the
  * pre-activation A . op(B) + bias, which gcn_act_grad_f32 wants.  A product of few tiles and a long k is cut along k, the
  * cuts' partial products go to the workspace and are added in order; query its size first (0 when one cut is enough;
- * 16-byte aligned).  ldc, ldr and ldp are at most 2^22 - 1. */
+ * 16-byte aligned).  ldc, ldr and ldp are at most 2^22 - 1; C must not overlap A, B or pre. */
 int gcn_gemm_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
                           int trans_b, const float* bias, int act, const float* residual, int64_t ldr, float* pre,

@@ -217,3 +217,12 @@ def test_operands_inside_matrices_of_nan(m, n, k, trans_b):
     for f in (lambda x, y: sparse.gemm_epilogue(x, y, trans_b=trans_b, act='silu'), lambda x, y: sparse.gemm(x, y, trans_b=trans_b),
               lambda x, y: sparse.gemm(x, y, trans_b=trans_b, relu=True)):
         assert torch.equal(f(va, vb), f(a, b))
+
+
+def test_a_result_over_an_operand_is_refused():
+    import torch
+    from gcn_amd import sparse
+    a, b = torch.randn((64, 64), device='cuda'), torch.randn((64, 64), device='cuda')
+    for out in (a, b):
+        with pytest.raises(ValueError):
+            sparse.gemm_epilogue(a, b, out=out)
