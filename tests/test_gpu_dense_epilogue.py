@@ -226,3 +226,33 @@ def test_a_result_over_an_operand_is_refused():
     for out in (a, b):
         with pytest.raises(ValueError):
             sparse.gemm_epilogue(a, b, out=out)
+
+
+@pytest.mark.parametrize('n,k', [(260, 40), (256, 64), (250, 40), (240, 8)])
+def test_element_offsets_past_32_bits(n, k):
+    """Nine million rows: 2^31 elements and more in the result, the residual and the pre-activation; sampled rows."""
+    import torch
+    from gcn_amd import sparse
+    m = 9000001
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip('needs 60 GB of free device memory')
+    gen = torch.Generator('cuda').manual_seed(n + k)
+    a = torch.empty((m, k), device='cuda').normal_(generator=gen)
+    b = torch.empty((k, n), device='cuda').normal_(generator=gen) / k ** 0.5
+    bias = torch.empty(n, device='cuda').normal_(generator=gen)
+    r = torch.empty((m, n), device='cuda').normal_(generator=gen)
+    out, pre = sparse.gemm_epilogue(a, b, bias=bias, act='gelu', residual=r, want_pre=True)
+    dz, db = sparse.act_grad(r, pre, 'gelu')
+    for lo in (0, (1 << 31) // n - 20, (1 << 30) // n - 20, m - 40):
+        rows = slice(lo, lo + 40)
+        _check(a[rows], b, False, bias, 'gelu', r[rows], out[rows], pre[rows])
+        _, s = _act(pre[rows].double(), 'gelu')
+        want = r[rows].double() * s
+        assert bool(((dz[rows].double() - want).abs() <= (26 + 2 * pre[rows].double().abs()) * U * r[rows].double().abs()).all())
+    total = torch.zeros(n, dtype=torch.float64, device='cuda')
+    size = torch.zeros(n, dtype=torch.float64, device='cuda')
+    for lo in range(0, m, 1 << 20):
+        total += dz[lo:lo + (1 << 20)].double().sum(0)
+        size += dz[lo:lo + (1 << 20)].double().abs().sum(0)
+    # at most m / 2048 rows of a group and a tree over the groups and workgroups: (4395 + 64) u of the magnitudes
+    assert bool(((db.double() - total).abs() <= 4500 * U * size).all())
