@@ -789,7 +789,7 @@ __global__ __launch_bounds__(kBlock) void spmm_long_reduce_kernel(int64_t n_long
         }
         if (relu) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = s[e] > 0.0f ? s[e] : 0.0f;
+            for (int e = 0; e < 4; ++e) s[e] = s[e] > 0.0f || (relu == kReluKeepNan && s[e] != s[e]) ? s[e] : 0.0f;
         }
         if (od.keep_prob < 1.0f) {
             const uint64_t id = (uint64_t)(od.index_offset + (int64_t)long_row[li] * od.pitch + j);

@@ -47,6 +47,8 @@ struct PlanView {
     const int64_t* long_chunk;
 };
 
+constexpr int kReluKeepNan = 2;      // launch_long_reduce's ReLU: 1 maps a NaN to 0, this one keeps it
+
 // the partial rows of the long rows of a table, added in chunk order into c (spmm.hip)
 int launch_long_reduce(const gcn_spmm_plan::LongTable& lt, int64_t f, const float* part, int64_t ldp, float* c, int64_t ldc,
                        int relu, int vec_c, hipStream_t st);

@@ -3,6 +3,8 @@
 //
 //   C[i, :] = act(sum_e (a_e s[col_e]) q[col_e, :])        float32 sums, one fused multiply-add an element
 //
+// The ReLU keeps a NaN (the float32 product's makes it 0): a row of B that stands for NaN as a whole stays visible.
+//
 // The product is bound by the rows it gathers: at 256 columns 256 bytes an entry (two 128-byte lines) and the entry's
 // scale, instead of the 1024 bytes of float32 rows.  A wave takes a strip of the rows the plan cut.  L lanes hold 16 columns
 // each (one 16-byte load a row), so 64 / L entries are gathered by one instruction; each lane group adds its entries, and at
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(kBlock, 6) void spmm_quant_kernel(PlanView pv, cons
         if (!(L < 4 && (lane & 3 & ~(L - 1)))) {                    // L = 1, 2: the groups past the fourth hold the same sum
 #pragma unroll
             for (int i = 0; i < kLeft; ++i)
-                if (act) acc[i] = acc[i] > 0.0f ? acc[i] : 0.0f;
+                if (act) acc[i] = acc[i] <= 0.0f ? 0.0f : acc[i];      // a NaN stays one
 #pragma unroll
             for (int i = 0; i < kLeft; i += 4) {
                 if (kLeft >= 4 && vec && at + i + 4 <= f) {
@@ -324,7 +326,7 @@ int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, con
     GCN_LAUNCH_CHECK();
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[1], st));
     if (lt.n_chunks > 0)
-        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu, c_vec && f % 4 == 0, st)) return rc;
+        if (int rc = launch_long_reduce(lt, f, part, ldp, c, ldc, relu ? kReluKeepNan : 0, c_vec && f % 4 == 0, st)) return rc;
     if (plan->timing) GCN_HIP_TRY(hipEventRecord(plan->ev[2], st));
     return GCN_OK;
 }

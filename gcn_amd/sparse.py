@@ -1103,7 +1103,7 @@ def rms_norm_grad(grad, h, weight, inv, grad_h=None, want_weight=True):
 
 def spmm_quant(a, q, relu=False, out=None):
     """``a @ B`` (optionally with ReLU) for the matrix B that the QuantRows ``q`` stand for, gathering their 8-bit rows.
-    float32 sums in a fixed order (not the serial order of ``spmm``).  The workspace of long rows belongs to the call, so
+    float32 sums in a fixed order (not the serial order of ``spmm``); the ReLU keeps a NaN.  The workspace of long rows belongs to the call, so
     products on several streams, or recorded in several graphs, do not share one; the plan of ``a`` is made at the first
     product (touch ``a.plan`` before recording)."""
     if not isinstance(q, QuantRows):

@@ -564,7 +564,8 @@ int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, c
 /* C[n_rows x f] = act(A . B) for B in 8-bit rows [n_cols rows of pitch ldq bytes, scales [n_cols]], f <= 32768: the
  * propagation step of gcn/layers.py:202 on a quarter of the bytes of gcn_spmm_csr_f32's operand.  Sums are float32; the
  * entries of a row are added in a fixed order that depends on the width (not the serial order of the float32 product),
- * long rows in the chunks of the wide product.  flags: GCN_RELU.  Workspace as for gcn_spmm_csr_f32. */
+ * long rows in the chunks of the wide product.  flags: GCN_RELU, which keeps a NaN here.  Workspace as for
+ * gcn_spmm_csr_f32. */
 int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, const int32_t* indices, const float* vals,
                            int64_t f, const uint8_t* q, int64_t ldq, const float* scales, float* c, int64_t ldc, int flags,
                            void* workspace, size_t workspace_bytes, void* stream);

@@ -212,3 +212,35 @@ def test_refusals():
                  lambda: sparse.spmm_quant(a, q, out=torch.empty((4, 20)))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize('f', [7, 40, 70, 256, 600])
+def test_relu_keeps_what_is_not_a_number(f):
+    """A row of B that stands for NaN as a whole makes its neighbours NaN under the ReLU too, rows summed in chunks and
+    their join among them; the others keep their bits."""
+    import torch
+    from gcn_amd import sparse
+    lengths = [5] * 40 + [3000, 1100, 2048]
+    a = _matrix(len(lengths), 300, lengths, 8)
+    a.indices[a.indices == 7] = 8                                   # row 7 is met by three rows only
+    a.indices[2], a.indices[200 + 2900], a.indices[200 + 3000] = 7, 7, 7
+    assert a.plan.n_chunks > 0
+    q = _rows(300, f, 9)
+    clean = sparse.spmm_quant(a, q, relu=True)
+    q.scales[7] = float('nan')
+    out = sparse.spmm_quant(a, q, relu=True)
+    hit = torch.zeros(a.n_rows, dtype=torch.bool, device='cuda')
+    hit[[0, 40, 41]] = True
+    assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit])
+
+
+def test_quant_dot_with_relu_shows_a_row_that_is_not_finite():
+    import torch
+    from gcn_amd import layers
+    n = 60
+    a = _matrix(n, n, [4] * n, 11)
+    x = torch.randn((n, 24), device='cuda')
+    x[13, 5] = float('inf')
+    out = layers.quant_dot(a, x, fuse_relu=True)
+    hit = (a.indices.view(n, 4) == 13).any(1)
+    assert bool(hit.any()) and bool(torch.isnan(out[hit]).all()) and bool(torch.isfinite(out[~hit]).all())
