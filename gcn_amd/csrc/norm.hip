@@ -26,21 +26,25 @@ namespace gcn {
 
 constexpr int kNormMaxF = 32768;
 constexpr int kWaveRowF = 1024;          // wider rows belong to a workgroup each
-// sum or maximum over the G lanes of a row (G <= 64: lanes of one wave; more: the workgroup, through `lds`)
+// the larger of two magnitudes, by their bits: a NaN is larger than everything
+__device__ __forceinline__ float larger(float a, float b) {
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+}
+// sum or largest magnitude over the G lanes of a row (G <= 64: lanes of one wave; more: the workgroup, through `lds`)
 template <int G, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* lds) {
     constexpr int W = G < 64 ? G : 64;
 #pragma unroll
     for (int d = W / 2; d > 0; d >>= 1) {
         const float o = __shfl_xor(v, d);
-        v = MAX ? fmaxf(v, o) : v + o;
+        v = MAX ? larger(v, o) : v + o;
     }
     if (G > 64) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
         v = lds[0];
 #pragma unroll
-        for (int w = 1; w < G / 64; ++w) v = MAX ? fmaxf(v, lds[w]) : v + lds[w];
+        for (int w = 1; w < G / 64; ++w) v = MAX ? larger(v, lds[w]) : v + lds[w];
     }
     return v;
 }
@@ -124,7 +128,7 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(v[j][e]));      // 0 past the row's end
+            for (int e = 0; e < 4; ++e) most = larger(most, fabsf(v[j][e]));      // 0 past the row's end
         most = row_reduce<G, true>(most, lds[2 * (t & 1) + 1]);
         float scale = fmaxf(most * (1.0f / kE4m3Max), kQuantScaleMin);
         // a row whose mean square or maximum is not finite has no scale: it stands for NaN as a whole

@@ -543,8 +543,8 @@ int gcn_quant_dense_f32(int64_t n_rows, int64_t f, const uint8_t* q, int64_t ldq
  * [n] (what gcn_rms_norm_grad_f32 wants), and one of
  *   y  [n x f] float32 (may be x or residual itself, but not h), or
  *   q, scales: y as 8-bit rows, scales[r] = max(max_c |y_c| / 448, 2^-120), q_c = e4m3(y_c / scales[r]) rounded to
- *   nearest even, the bytes up to the next multiple of 16 zero.  A row whose mean square or maximum is not finite gets
- *   the scale NaN and stands for NaN as a whole.
+ *   nearest even, the bytes up to the next multiple of 16 zero.  A row whose mean square or maximum is not finite (a
+ *   weight that is not makes every row such a one) gets the scale NaN and stands for NaN as a whole.
  * Sums are float32: a row whose sum of squares exceeds the float32 range has inv = 0. */
 int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const float* residual, int64_t ldr,
                      const float* weight, float eps, float* h, int64_t ldh, float* inv, float* y, int64_t ldy,

@@ -263,3 +263,18 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
     assert np.isfinite(sparse.rms_norm(x, w)[0].cpu().numpy()).all()
+
+
+@pytest.mark.parametrize('f', [7, 64, 300, 1500, 17003])
+def test_a_weight_that_is_not_finite_makes_whole_rows_nan(f):
+    """The maximum of a row with a NaN in it is no number: the row's scale is NaN, as where the row itself is not finite."""
+    import torch
+    from gcn_amd import sparse
+    x = torch.randn((9, f), device='cuda')
+    x[4, f - 1] = 0.0                                              # 0 * inf is NaN as well
+    for bad in (float('nan'), float('inf'), -float('inf')):
+        for at in (0, f // 2, f - 1):
+            w = torch.ones(f, device='cuda')
+            w[at] = bad
+            q = sparse.rms_norm(x, w, quant=True)[0]
+            assert bool(torch.isnan(q.scales).all()) and bool(torch.isnan(q.dense()).all())
