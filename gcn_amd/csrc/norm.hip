@@ -130,10 +130,12 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) most = larger(most, fabsf(v[j][e]));      // 0 past the row's end
         most = row_reduce<G, true>(most, lds[2 * (t & 1) + 1]);
-        float scale = fmaxf(most * (1.0f / kE4m3Max), kQuantScaleMin);
+        // Quotients, not products with a rounded inverse: those put the scale of six rows in ten one step off and now and
+        // then a byte on the wrong side of the middle of two.  Within 1 % of the products' time up to 16,384 columns, where
+        // the memory hides them; past that, a workgroup a compute unit, 8 % (8192 x 32,768: 773 -> 836 us).
+        float scale = fmaxf(most / kE4m3Max, kQuantScaleMin);
         // a row whose mean square or maximum is not finite has no scale: it stands for NaN as a whole
         if (!(ms < INFINITY) || !(most < INFINITY)) scale = NAN;
-        const float up = 1.0f / scale;
         if (live && sub == 0) a.scales[i] = scale;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_kernel(NormArgs a, int tile) {
             // the bytes from f to the next multiple of 16 are part of the row and zero
             if (live && c < ((f + 15) & ~15))
                 *reinterpret_cast<uint32_t*>(a.q + i * a.ldq + c) =
-                    e4m3_pack4(v[j][0] * up, v[j][1] * up, v[j][2] * up, v[j][3] * up, f - c);
+                    e4m3_pack4(v[j][0] / scale, v[j][1] / scale, v[j][2] / scale, v[j][3] / scale, f - c);
         }
     }
 }

@@ -278,3 +278,17 @@ def test_a_weight_that_is_not_finite_makes_whole_rows_nan(f):
             w[at] = bad
             q = sparse.rms_norm(x, w, quant=True)[0]
             assert bool(torch.isnan(q.scales).all()) and bool(torch.isnan(q.dense()).all())
+
+
+@pytest.mark.parametrize('n,f', [(4000, 16), (3000, 100), (2000, 256), (1500, 500), (700, 1433), (90, 5001), (40, 9000), (30, 20001)])
+def test_bytes_are_the_quotients_by_the_scale(n, f):
+    """Scale and bytes as they are defined, with no rounding more: the float32 output (the same y) divided by 448 and by the
+    scale, IEEE division on the host, rounded to nearest even.  Equal bit for bit."""
+    import torch
+    from gcn_amd import sparse
+    x, r, w, _, _ = _inputs(n, f, 7)
+    q = sparse.rms_norm(x, w, residual=r, quant=True)[0]
+    y = sparse.rms_norm(x, w, residual=r)[0].cpu()
+    scale = (y.abs().amax(1) / 448.0).clamp(min=2.0 ** -120)
+    assert torch.equal(q.scales.cpu(), scale)
+    assert torch.equal(q.data[:, :f].cpu(), (y / scale[:, None]).to(torch.float8_e4m3fn).view(torch.uint8))
