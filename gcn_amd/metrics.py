@@ -28,7 +28,8 @@ class _DistillationFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, preds, values, indices, mask, mask_mean, temperature):
         stats, _ = sparse.distill_topk(preds, values, indices, mask, mask_mean, temperature=temperature, want_grad=False)
-        loss, agreement = sparse.loss_summary(stats, None, 0.0).unbind()
+        with sparse._on_device(stats):        # loss_summary enqueues on the current device's stream
+            loss, agreement = sparse.loss_summary(stats, None, 0.0).unbind()
         ctx.save_for_backward(preds, values, indices, mask)
         ctx.mask_mean, ctx.temperature = mask_mean, temperature
         ctx.mark_non_differentiable(agreement)

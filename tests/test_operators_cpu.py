@@ -187,3 +187,32 @@ def test_calls_go_to_the_device_of_their_tensors(monkeypatch):
         sparse._on_device(OnGpu(0), torch.ones(1))
     with pytest.raises(ValueError):
         sparse._on_device(torch.ones(1))
+
+
+def test_the_distillation_loss_is_averaged_on_the_device_of_its_rows(monkeypatch):
+    """With another GPU current, the rows' mean is enqueued where the rows are."""
+    import contextlib
+    import torch
+    from gcn_amd import metrics, sparse
+    current, calls = ['cuda:0'], []
+
+    @contextlib.contextmanager
+    def on_device(first, *others):
+        before, current[0] = current[0], 'cuda:1'
+        yield
+        current[0] = before
+
+    def distill(preds, *args, **kwargs):
+        with sparse._on_device(preds):
+            calls.append(('rows', current[0]))
+        return torch.zeros((preds.shape[0], 2)), None
+
+    def summary(stats, weights, decay):
+        calls.append(('mean', current[0]))
+        return torch.zeros(2)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(sparse, '_on_device', on_device)
+    monkeypatch.setattr(sparse, 'distill_topk', distill)
+    monkeypatch.setattr(sparse, 'loss_summary', summary)
+    metrics.masked_distillation(torch.zeros(3, 4), torch.zeros(3, 2), torch.zeros((3, 2), dtype=torch.int32), mask_mean=1.0)
+    assert calls == [('rows', 'cuda:1'), ('mean', 'cuda:1')] and current == ['cuda:0']
