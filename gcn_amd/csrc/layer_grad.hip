@@ -14,9 +14,11 @@ namespace gcn {
 
 constexpr int kTileCols = 256;           // columns of a workgroup; wider matrices take more of them (grid y)
 
+// dz may be dout or pre itself (no __restrict__ on the three): a lane reads its columns of a row before it stores them, and
+// what a shifted load of a row's last columns takes besides them is replaced.
 template <int G>
-__global__ __launch_bounds__(256) void act_grad_kernel(int64_t m, int n, int act, const float* __restrict__ dout, int64_t ldo,
-                                                       const float* __restrict__ pre, int64_t ldp, float* dz, int64_t ldz,
+__global__ __launch_bounds__(256) void act_grad_kernel(int64_t m, int n, int act, const float* dout, int64_t ldo,
+                                                       const float* pre, int64_t ldp, float* dz, int64_t ldz,
                                                        float* __restrict__ part, int64_t tile) {
     constexpr int kRows = 256 / G;
     __shared__ float cols[kRows > 1 ? (kRows - 1) * G * 4 : 1];

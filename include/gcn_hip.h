@@ -553,7 +553,7 @@ int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const fl
 /* Gradients of it (of the values y stands for when it was written in 8 bits): with g = weight * dy
  *   dx_c = dh_c + inv * (g_c - h_c * inv^2 * mean_c(g h))     -- the gradient of x and of the residual alike
  *   dweight_c = sum over rows of dy_c * h_c * inv
- * dh (may be NULL): the gradient that reaches h itself, for a layer that hands h on.  dx (may be dy or dh itself) or
+ * dh (may be NULL): the gradient that reaches h itself, for a layer that hands h on.  dx (may be dy, dh or h itself) or
  * dweight may be NULL.  The rows of dweight are summed in a fixed order; workspace (16-byte aligned) as the query
  * says, not needed without dweight. */
 int gcn_rms_norm_grad_workspace_bytes(int64_t n, int64_t f, size_t* bytes);
@@ -580,7 +580,7 @@ int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64
                           int trans_b, const float* bias, int act, const float* residual, int64_t ldr, float* pre,
                           int64_t ldp, float* c, int64_t ldc, void* workspace, size_t workspace_bytes, void* stream);
 
-/* The part of its backward pass that is no product: dz = dout * act'(pre) (may be dout itself; NULL: not wanted) and
+/* The part of its backward pass that is no product: dz = dout * act'(pre) (may be dout or pre itself; NULL: not wanted) and
  * dbias [n] (may be NULL) = the sum of dz over the rows, in a fixed order.  pre is not read for GCN_ACT_NONE.  The gradients
  * of A, B and the residual are gcn_gemm_f32 (trans_b swapped) and gcn_gemm_tn_f32 on dz, and dout.  Workspace (16-byte
  * aligned) as the query says, not needed without dbias. */
