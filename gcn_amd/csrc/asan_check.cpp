@@ -2,13 +2,14 @@
 // sources are compiled into ONE executable with AddressSanitizer and UndefinedBehaviorSanitizer on the host
 // code (device code is built as usual and never runs here).  It needs no GPU: it walks the host-only parts of
 // the C ABI -- the size queries, the argument validation of every entry point, which returns before any HIP
-// call, the error text -- and the host half of plan creation (the long-row tables) on random row lengths.
+// call, the error text --, the check of overlapping operands and the host half of plan creation (the long-row tables) on random row lengths.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <random>
 
 #include "common.h"
+#include "operands.h"
 
 static int g_failures = 0;
 #define EXPECT(cond)                                                          \
@@ -44,6 +45,43 @@ static void size_queries() {
     EXPECT(gcn_coo_to_csr_bound(-1, 0, 0, &cap, &bytes) == GCN_ERR_BAD_ARG);
     EXPECT(gcn_coo_to_csr_bound(1, 1, 0, nullptr, &bytes) == GCN_ERR_BAD_ARG);
     EXPECT(gcn_version() >= 100 && strlen(gcn_build_hash()) == 64);
+}
+
+// share_memory against the bytes themselves: small matrices at every kind of distance and pitch
+static void places() {
+    uint64_t state = 7;
+    auto draw = [&](int n) { return (int)((state = gcn::sm64(state)) % (uint64_t)n); };
+    static const uint8_t memory[1] = {0};
+    for (int t = 0; t < 200000; ++t) {
+        int rows[2], width[2], pitch[2], at[2];
+        std::vector<uint8_t> owner(4096, 0);
+        bool want = false;
+        for (int k = 0; k < 2; ++k) {
+            rows[k] = draw(9);
+            width[k] = 1 + draw(8);
+            pitch[k] = width[k] + draw(12);
+            at[k] = draw(120);
+        }
+        if (t % 2) pitch[1] = std::max(pitch[0], width[1]);
+        for (int k = 0; k < 2; ++k)
+            for (int r = 0; r < rows[k]; ++r)
+                for (int c = 0; c < width[k]; ++c) {
+                    uint8_t& o = owner[at[k] + r * pitch[k] + c];
+                    want = want || (k == 1 && o == 1);
+                    if (k == 0) o = 1;
+                }
+        const gcn::Place a = gcn::place((const uint8_t*)((uintptr_t)memory + at[0]), rows[0], width[0], pitch[0]);
+        const gcn::Place b = gcn::place((const uint8_t*)((uintptr_t)memory + at[1]), rows[1], width[1], pitch[1]);
+        EXPECT(gcn::share_memory(a, b) == want && gcn::share_memory(b, a) == want);
+    }
+    // two row ranges of a large matrix, and its two halves of columns
+    const float* base = (const float*)(uintptr_t)4096;
+    const int64_t n = (int64_t)1 << 31;
+    EXPECT(!gcn::share_memory(gcn::place(base, n, 100, 256), gcn::place(base + 100, n, 156, 256)));
+    EXPECT(gcn::share_memory(gcn::place(base, n, 101, 256), gcn::place(base + 100, n, 156, 256)));
+    EXPECT(!gcn::share_memory(gcn::place(base, n, 256, 256), gcn::place(base + n * 256, n, 256, 256)));
+    EXPECT(gcn::share_memory(gcn::place(base, n, 256, 256), gcn::place(base + n * 256 - 1, n, 256, 256)));
+    EXPECT(!gcn::share_memory(gcn::place((const float*)nullptr, n, 4, 4), gcn::place((const float*)nullptr, n, 4, 4)));
 }
 
 static void argument_validation() {
@@ -258,6 +296,7 @@ static void long_row_tables() {
 
 int main() {
     size_queries();
+    places();
     argument_validation();
     dropout_thresholds();
     long_row_tables();

@@ -6,6 +6,7 @@
 
 #include "activations.h"
 #include "common.h"
+#include "operands.h"
 
 namespace gcn {
 
@@ -1709,7 +1710,13 @@ int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64
     const size_t need = cuts > 1 ? (size_t)cuts * (size_t)m * (size_t)n * sizeof(float) : 0;
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
-    if (c && (c == a || c == b || c == pre)) return fail(GCN_ERR_BAD_ARG, "the result needs memory of its own");
+    const Place in_a = place(k ? a : nullptr, m, k, lda), in_b = place(k ? b : nullptr, trans_b ? n : k, trans_b ? k : n, ldb);
+    const Place in_bias = place(bias, n), in_r = place(residual, m, n, ldr), out_c = place(c, m, n, ldc), out_p = place(pre, m, n, ldp);
+    for (const Place& out : {out_c, out_p})
+        if (share_memory(out, in_a) || share_memory(out, in_b) || share_memory(out, in_bias))
+            return fail(GCN_ERR_BAD_ARG, "the result or pre lies over A, B or the bias: it needs memory of its own");
+    if (share_memory(out_c, out_p) || share_memory(out_p, in_r) || lies_across(out_c, in_r))
+        return fail(GCN_ERR_BAD_ARG, "the result and pre need memory of their own: only the result may be the residual itself");
     if (cuts > 1) {
         if (int rc = n <= 32   ? launch_cuts<32>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)
                      : n <= 64 ? launch_cuts<64>(m, n, k, cuts, a, lda, b, ldb, trans_b, (float*)workspace, st)

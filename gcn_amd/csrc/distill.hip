@@ -17,6 +17,7 @@
 
 #include "common.h"
 #include "lanes.h"
+#include "operands.h"
 #include "row_vectors.h"
 
 namespace gcn {
@@ -586,12 +587,18 @@ int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx,
     if (!(temperature > 0.0f) || !(temperature < INFINITY)) return fail(GCN_ERR_BAD_ARG, "the temperature must be positive");
     if (n == 0) return GCN_OK;
     if (!logits || !values || !indices) return fail(GCN_ERR_BAD_ARG, "null pointer");
-    if (dlogits == logits) return fail(GCN_ERR_BAD_ARG, "the gradient needs memory of its own: the logits are read after its first stores");
     if (row_stats && ((uintptr_t)row_stats & 7)) return fail(GCN_ERR_BAD_ARG, "row_stats must be 8-byte aligned");
     if (!row_stats && !dlogits) return GCN_OK;
+    const int64_t value_size = value_type == GCN_F32 ? 4 : 2;
+    const Place out_d = place(dlogits, n, c, ldd), out_s = place(row_stats, n, 2, 2);
+    const Place in[] = {place(logits, n, c, ldx), place((const char*)values, n, k * value_size, ldv * value_size),
+                        place(indices, n, k, ldi), place(mask, n), place(upstream, 1)};
+    for (const Place& operand : in)
+        if (share_memory(out_d, operand) || share_memory(out_s, operand))
+            return fail(GCN_ERR_BAD_ARG, "an output lies over an operand: it needs memory of its own, the operands are read after its first stores");
+    if (share_memory(out_d, out_s)) return fail(GCN_ERR_BAD_ARG, "two outputs share memory: each needs its own");
     // a launch counts its threads in 32 bits: rows of at most 64 threads, or of up to 1024
     const int64_t slice = (c <= kWaveRowC ? (int64_t)1 << 26 : (int64_t)1 << 22) - 4;
-    const int64_t value_size = value_type == GCN_F32 ? 4 : 2;
     for (int64_t r = 0; r < n; r += slice) {
         const DistillArgs a = {std::min(slice, n - r), 1.0f / (float)n, (int)c, logits + r * ldx, ldx,
                                (const char*)values + r * ldv * value_size, value_type, ldv, indices + r * ldi, ldi, (int)k,

@@ -8,6 +8,7 @@
 
 #include "activations.h"
 #include "common.h"
+#include "operands.h"
 #include "row_vectors.h"
 
 namespace gcn {
@@ -130,6 +131,10 @@ int gcn_act_grad_f32(int64_t m, int64_t n, int act, const float* dout, int64_t l
         if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
             return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
     }
+    const Place out = place(dz, m, n, ldz);
+    if (lies_across(out, place(dout, m, n, ldo)) || (act != GCN_ACT_NONE && lies_across(out, place(pre, m, n, ldp))) ||
+        share_memory(out, place(dbias, n)))
+        return fail(GCN_ERR_BAD_ARG, "dz lies across dout, pre or dbias: it may be dout or pre itself");
     const dim3 grid((unsigned)blocks, (unsigned)ceil_div(n, (int64_t)kTileCols));
     if (grid.y > 65535) return fail(GCN_ERR_BAD_ARG, "too many columns for one launch");
 #define GCN_ACT_GO(G)                                                                                                       \

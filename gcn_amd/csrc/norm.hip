@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "operands.h"
 #include "quant_rows.h"
 #include "row_vectors.h"
 
@@ -418,7 +419,20 @@ int gcn_rms_norm_f32(int64_t n, int64_t f, const float* x, int64_t ldx, const fl
     if (n == 0) return GCN_OK;
     if ((y != nullptr) == (q != nullptr)) return fail(GCN_ERR_BAD_ARG, "one of the outputs y and q is wanted");
     if (!x || !inv || (residual && !h)) return fail(GCN_ERR_BAD_ARG, "null pointer");
-    if (y && residual && y == h) return fail(GCN_ERR_BAD_ARG, "y and h are two outputs: they need memory of their own");
+    const Place in_x = place(x, n, f, ldx), in_r = place(residual, n, f, ldr), in_w = place(weight, f);
+    const Place out_h = place(residual ? h : nullptr, n, f, ldh), out_y = place(y, n, f, ldy);
+    const Place out_q = place(q, n, (f + 15) / 16 * 16, ldq), out_i = place(inv, n), out_s = place(q ? scales : nullptr, n);
+    for (const Place& out : {out_h, out_y})
+        if (lies_across(out, in_x) || lies_across(out, in_r) || share_memory(out, in_w))
+            return fail(GCN_ERR_BAD_ARG, "an output lies across x, the residual or the weight: it may be x or the residual itself");
+    for (const Place& out : {out_q, out_i, out_s})
+        if (share_memory(out, in_x) || share_memory(out, in_r) || share_memory(out, in_w))
+            return fail(GCN_ERR_BAD_ARG, "inv, q or the scales lie over an operand");
+    const Place outs[] = {out_h, out_y, out_q, out_i, out_s};
+    for (int i = 0; i < 5; ++i)
+        for (int j = 0; j < i; ++j)
+            if (share_memory(outs[i], outs[j]))
+                return fail(GCN_ERR_BAD_ARG, "two outputs share memory: each needs its own");
     NormArgs a = {n, (int)f, x, ldx, residual, ldr, weight, eps, h, ldh, inv, y, ldy, q, ldq, scales};
     const int tile = norm_tile(n, f);
     const int64_t blocks = ceil_div(n, (int64_t)norm_rows(f) * tile);
@@ -455,6 +469,10 @@ int gcn_rms_norm_grad_f32(int64_t n, int64_t f, const float* dy, int64_t lddy, c
         if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
             return fail(GCN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed (16-byte aligned)", workspace_bytes, need);
     }
+    const Place out = place(dx, n, f, lddx);
+    if (lies_across(out, place(dy, n, f, lddy)) || lies_across(out, place(h, n, f, ldh)) || lies_across(out, place(dh, n, f, lddh)) ||
+        share_memory(out, place(weight, f)) || share_memory(out, place(inv, n)) || share_memory(out, place(dweight, f)))
+        return fail(GCN_ERR_BAD_ARG, "dx lies across an operand or dweight: it may be dy, dh or h itself");
     NormGradArgs a = {n, (int)f, dy, lddy, h, ldh, weight, inv, dh, lddh, dx, lddx, dweight ? (float*)workspace : nullptr};
     const int tile = (int)norm_grad_tile(n, f);
 #define GCN_LAUNCH_NORM(G, VPL, BLOCK) \

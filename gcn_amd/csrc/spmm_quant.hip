@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "operands.h"
 #include "quant_rows.h"
 #include "spmm_plan.h"
 
@@ -264,6 +265,9 @@ int gcn_quant_dense_f32(int64_t n_rows, int64_t f, const uint8_t* q, int64_t ldq
     if (n_rows == 0) return GCN_OK;
     if (!q || !scales || !y) return fail(GCN_ERR_BAD_ARG, "null pointer");
     if (!aligned16(q)) return fail(GCN_ERR_BAD_ARG, "8-bit rows must be 16-byte aligned");
+    if (share_memory(place(y, n_rows, f, ldy), place(q, n_rows, (f + 15) / 16 * 16, ldq)) ||
+        share_memory(place(y, n_rows, f, ldy), place(scales, n_rows)))
+        return fail(GCN_ERR_BAD_ARG, "y lies over the 8-bit rows or their scales");
     const int64_t blocks = std::min<int64_t>(ceil_div(n_rows * ((f + 3) / 4), (int64_t)kBlock), 1 << 16);
     quant_dense_kernel<<<(unsigned)blocks, kBlock, 0, (hipStream_t)stream>>>(n_rows, (int)f, q, ldq, scales, y, ldy);
     GCN_LAUNCH_CHECK();
@@ -308,6 +312,9 @@ int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, con
     }
     const int64_t grid = pv.chunk_blocks + ceil_div(plan->n_strips, kWaves);
     if (grid >= (int64_t)1 << 24) return fail(GCN_ERR_BAD_ARG, "matrix too large for one launch");   // threads count in 32 bits
+    const Place out = place(c, plan->n_rows, f, ldc);
+    if (share_memory(out, place(q, plan->n_cols, (f + 15) / 16 * 16, ldq)) || share_memory(out, place(scales, plan->n_cols)))
+        return fail(GCN_ERR_BAD_ARG, "the result lies over the 8-bit rows or their scales");
     hipStream_t st = (hipStream_t)stream;
     const int relu = (flags & GCN_RELU) ? 1 : 0;
     const int c_vec = (ldc % 4 == 0 && aligned16(c)) ? 1 : 0;

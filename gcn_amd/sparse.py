@@ -1035,8 +1035,8 @@ class QuantRows(object):
 def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=False, out=None, sum_out=None):
     """``(y, h, inv)`` with ``h = x + residual`` (``x`` itself without a residual), ``inv = 1 / sqrt(mean(h^2) + eps)``
     of every row and ``y = h * inv * weight``: float32, or QuantRows with ``quant``.  One pass over the rows.
-    ``out``: where ``y`` goes (a float32 view, or QuantRows); ``sum_out``: where ``h`` goes, which may be ``x`` or
-    ``residual`` itself (``y`` and ``h`` need memory of their own).  A row holds at most 32768 columns.  ``h`` and
+    ``out``: where ``y`` goes (a float32 view, or QuantRows); ``sum_out``: where ``h`` goes; either may be ``x`` or
+    ``residual`` itself, but lie over them in no other way (``y`` and ``h`` need memory of their own).  A row holds at most 32768 columns.  ``h`` and
     ``inv`` are what ``rms_norm_grad`` wants."""
     with _on_device(x, weight, residual, sum_out):
         x = _matrix(x)

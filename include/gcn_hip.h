@@ -528,6 +528,10 @@ int gcn_adam_f32(int64_t n, float* param, const float* grad, float* m, float* v,
  * (gcn/layers.py:183-214) and its loss (gcn/metrics.py:85-101).                *
  * ------------------------------------------------------------------------- */
 
+/* In these calls an output shares memory with no operand and with no other output; where one "may be" an operand "itself",
+ * it is the same rows at the same address and leading dimension.  Anything else is refused (GCN_ERR_BAD_ARG).  Columns of
+ * one wider matrix beside each other share nothing. */
+
 /* 8-bit rows with a scale each: element (r, c) is scales[r] * e4m3(q[r * ldq + c]).  The pitch ldq is a multiple of 16
  * bytes, the address 16-byte aligned, and the bytes from f to the next multiple of 16 belong to the row and are zero.
  * gcn_quant_pitch: the pitch to allocate for f <= 32768 columns -- a power of two up to 128 bytes, then a multiple
@@ -541,7 +545,7 @@ int gcn_quant_dense_f32(int64_t n_rows, int64_t f, const uint8_t* q, int64_t ldq
  *   h = x + residual (x itself if residual is NULL),  inv = 1 / sqrt(mean_c h_c^2 + eps),  y_c = h_c * inv * weight_c
  * (weight NULL: all ones), f <= 32768 columns.  Written: h (only with a residual; may be x or residual itself), inv
  * [n] (what gcn_rms_norm_grad_f32 wants), and one of
- *   y  [n x f] float32 (may be x or residual itself, but not h), or
+ *   y  [n x f] float32 (may be x or residual itself), or
  *   q, scales: y as 8-bit rows, scales[r] = max(max_c |y_c| / 448, 2^-120), q_c = e4m3(y_c / scales[r]) rounded to
  *   nearest even, the bytes up to the next multiple of 16 zero.  A row whose mean square or maximum is not finite (a
  *   weight that is not makes every row such a one) gets the scale NaN and stands for NaN as a whole.
@@ -574,7 +578,7 @@ int gcn_spmm_csr_quant_f32(const gcn_spmm_plan* plan, const int64_t* indptr, con
  * epilogue in its store.  bias [n], residual [m x n] (may be C itself) and pre may be NULL; pre [m x n] receives the
  * pre-activation A . op(B) + bias, which gcn_act_grad_f32 wants.  A product of few tiles and a long k is cut along k, the
  * cuts' partial products go to the workspace and are added in order; query its size first (0 when one cut is enough;
- * 16-byte aligned).  ldc, ldr and ldp are at most 2^22 - 1; C must not overlap A, B or pre. */
+ * 16-byte aligned).  ldc, ldr and ldp are at most 2^22 - 1. */
 int gcn_gemm_epilogue_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int gcn_gemm_epilogue_f32(int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
                           int trans_b, const float* bias, int act, const float* residual, int64_t ldr, float* pre,
@@ -595,7 +599,7 @@ int gcn_act_grad_f32(int64_t m, int64_t n, int act, const float* dout, int64_t l
  *   row_stats [n x 2] (may be NULL, 8-byte aligned): (T^2 sum_j p_j (log p_j - log q_idx_j) * w_i,
  *       w_i where the row's first maximum is the class of the largest listed logit -- of equal ones the first listed --,
  *       else 0): the rows gcn_loss_summary_f32 averages
- *   dlogits [n x c] (may be NULL; must not overlap the logits): (q_c - P_c) * T * w_i / n [* *upstream], P_c the sum of
+ *   dlogits [n x c] (may be NULL): (q_c - P_c) * T * w_i / n [* *upstream], P_c the sum of
  *       the p_j listed at class c.  upstream (device scalar, may be NULL) is read when the kernel runs.
  * Rows with mask 0 are not read and rows without an entry (or with listed logits of -inf only) have no loss: both get
  * zeros.  A NaN or +inf in a row of the mask makes that row NaN; a logit of -inf at a listed class makes its loss +inf. */

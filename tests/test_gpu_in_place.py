@@ -88,3 +88,37 @@ def test_norm_over_x_and_the_residual(f):
         both = [x.clone(), r.clone()]
         y2, h2, inv2 = sparse.rms_norm(both[0], w, residual=both[1], out=both[y_over], sum_out=both[1 - y_over])
         assert torch.equal(y2, y) and torch.equal(h2, h) and torch.equal(inv2, inv)
+
+
+def test_views_of_one_buffer():
+    """Shifted rows are refused by the Python operators; columns beside each other in one wider matrix are memory of their
+    own and give the results of separate matrices."""
+    import torch
+    from gcn_amd import sparse
+    n, f = 50, 24
+    buf = torch.randn((n + 1, f), device='cuda')
+    r, w, b = torch.randn((n, f), device='cuda'), torch.rand(f, device='cuda'), torch.randn((f, f), device='cuda')
+    rows = sparse.QuantRows(n, f, torch.zeros((n, 32), dtype=torch.uint8, device='cuda'), torch.ones(n, device='cuda'))
+    flat = rows.data.flatten().view(torch.float32)
+    for call in (lambda: sparse.rms_norm(buf[:n], w, out=buf[1:]), lambda: sparse.rms_norm(buf[1:], w, out=buf[:n]),
+                 lambda: sparse.rms_norm(buf[:n], w, residual=r, sum_out=buf[1:]),
+                 lambda: sparse.rms_norm(r, w, residual=r, sum_out=buf[:n], out=buf[1:]),
+                 lambda: sparse.gemm_epilogue(buf[:n], b, out=buf[1:]), lambda: sparse.gemm_epilogue(r, b, residual=buf[:n], out=buf[1:]),
+                 lambda: sparse.gemm_epilogue(b[:, :8].contiguous(), b[:8], out=b),
+                 lambda: rows.rows(0, 8).dense(out=flat[:8 * f].view(8, f))):
+        with pytest.raises(ValueError):
+            call()
+    wide = torch.randn((n, 3 * f), device='cuda')
+    x, h, y = wide[:, :f], wide[:, f:2 * f], wide[:, 2 * f:]
+    want_y, want_h, _ = sparse.rms_norm(x.contiguous(), w, residual=r)
+    sparse.rms_norm(x, w, residual=r, out=y, sum_out=h)
+    assert torch.equal(y, want_y) and torch.equal(h, want_h)
+    want = sparse.gemm_epilogue(x.contiguous(), b, act='silu', residual=h.contiguous())
+    assert torch.equal(sparse.gemm_epilogue(x, b, act='silu', residual=h, out=y), want)
+    a = sparse.DeviceCSR(n, n, torch.arange(n + 1, device='cuda'), torch.arange(n, dtype=torch.int32, device='cuda'), torch.ones(n, device='cuda'))
+    block = torch.zeros((n, 256), dtype=torch.uint8, device='cuda')
+    q = sparse.rms_norm(r, w, quant=True, out=sparse.QuantRows(n, f, block[:, :32], torch.empty(n, device='cuda')))[0]
+    beside = block.view(torch.float32)[:, 16:16 + f]
+    assert torch.equal(sparse.spmm_quant(a, q, out=beside), q.dense())
+    with pytest.raises(ValueError):
+        sparse.spmm_quant(a, q, out=block.view(torch.float32)[:, 4:4 + f])

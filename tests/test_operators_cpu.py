@@ -216,3 +216,43 @@ def test_the_distillation_loss_is_averaged_on_the_device_of_its_rows(monkeypatch
     monkeypatch.setattr(sparse, 'loss_summary', summary)
     metrics.masked_distillation(torch.zeros(3, 4), torch.zeros(3, 2), torch.zeros((3, 2), dtype=torch.int32), mask_mean=1.0)
     assert calls == [('rows', 'cuda:1'), ('mean', 'cuda:1')] and current == ['cuda:0']
+
+
+def test_outputs_across_operands_are_refused():
+    """Shifted views of one buffer: where operand and result, or two results, share rows otherwise than row by row, the call
+    is refused before any launch.  4 rows of 6 columns are 96 bytes; addresses far apart stand for memory of its own."""
+    X, R, W, H, Y, Q, S, I = (P + (k << 16) for k in range(1, 9))
+    need = ctypes.c_size_t()
+    lib = _lib()
+
+    def norm(**kw):
+        return _norm(**dict(dict(x=X, r=R, ldr=6, h=H, inv=I, y=Y), **kw))
+    for bad in (dict(y=X + 24), dict(y=X - 24), dict(y=X + 92), dict(y=R - 4), dict(y=H + 24), dict(y=H - 92), dict(y=X, ldy=7),
+                dict(h=X + 24), dict(h=R, ldh=8), dict(inv=X + 80), dict(inv=Y), dict(inv=H + 4),
+                dict(y=None, q=X, ldq=16, scales=S), dict(y=None, q=H + 80, ldq=16, scales=S), dict(y=None, q=Q, ldq=16, scales=Q + 48),
+                dict(y=None, q=Q, ldq=16, scales=I + 12), dict(y=None, q=Q, ldq=16, scales=R)):
+        assert norm(**bad) == BAD and b'null' not in lib.gcn_last_error_string(), bad
+    assert lib.gcn_rms_norm_f32(4, 6, X, 6, None, 0, W, 1e-6, None, 6, I, W - 72, 6, None, 0, None, None) == BAD
+    for bad in (dict(dx=X + 24), dict(dx=H - 92), dict(dx=R + 4, dh=R, lddh=6), dict(dx=X, lddx=9), dict(dx=I + 8)):
+        assert _norm_grad(**dict(dict(dy=X, h=H, inv=I), **bad)) == BAD, bad
+    assert lib.gcn_rms_norm_grad_workspace_bytes(4, 6, ctypes.byref(need)) == 0
+    assert _norm_grad(dy=X, h=H, inv=I, dx=Y, dw=Y + 72, ws=Q, nbytes=need.value) == BAD
+
+    def dense(**kw):
+        return _dense(**dict(dict(a=X, b=W, bias=S, r=R, pre=H, c=Y), **kw))
+    for bad in (dict(c=X), dict(c=X + 92), dict(c=X - 76), dict(c=W + 100), dict(c=W + 116), dict(c=H + 20), dict(c=H - 4), dict(c=R + 20),
+                dict(c=R, ldc=6), dict(c=S), dict(pre=X + 4), dict(pre=W), dict(pre=R), dict(pre=S - 76),
+                dict(tb=1, ldb=6, c=W + 116)):
+        assert dense(**bad) == BAD, bad
+    for bad in (dict(dz=X + 20), dict(dz=X, ldz=7), dict(dz=H - 20), dict(dz=H + 76)):
+        assert _act_grad(**dict(dict(g=X, pre=H), **bad)) == BAD, bad
+    assert lib.gcn_act_grad_workspace_bytes(4, 5, ctypes.byref(need)) == 0
+    assert _act_grad(g=X, pre=H, dz=Y, db=Y + 60, ws=Q, nb=need.value) == BAD
+
+    def distill(**kw):
+        return _distill(**dict(dict(x=X, v=R, i=W, mask=S, stats=I, d=Y), **kw))
+    for bad in (dict(d=X), dict(d=X + 24), dict(d=X - 92), dict(d=R + 44), dict(d=W - 8), dict(d=S + 12), dict(stats=X + 88),
+                dict(stats=Y + 88), dict(stats=S), dict(up=Y + 4)):
+        assert distill(**bad) == BAD, bad
+    assert lib.gcn_quant_dense_f32(4, 6, Q, 16, S, Q + 60, 6, None) == BAD
+    assert lib.gcn_quant_dense_f32(4, 6, Q, 16, S, S - 88, 6, None) == BAD
