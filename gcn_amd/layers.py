@@ -4,6 +4,9 @@
 names and defaults.  Every product runs in ``libgcn_hip.so``; torch supplies memory, streams
 and the autograd tape.
 """
+import functools
+import os
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -149,16 +152,47 @@ class _GatedGemmFn(torch.autograd.Function):
 _MARKED_BELOW = frozenset(('_RmsNormFnBackward', '_QuantDotFnBackward', '_DenseFnBackward'))
 
 
+def _refuse_eager_graph():
+    raise RuntimeError('an eager autograd graph over an input of this recorded call is alive: drop its outputs and losses '
+                       'before capturing')
+
+
+def _records(device, stream_id):
+    """Whether a stream takes part in a recording (the default stream, number 0, cannot)."""
+    if stream_id == 0:
+        return False
+    current = torch.cuda.current_stream()
+    if (device, stream_id) == (current.device_index, current.stream_id):
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(torch.cuda.Stream(stream_id=stream_id, device_index=device, device_type=current.device_type)):
+        return torch.cuda.is_current_stream_capturing()
+
+
+@functools.lru_cache(maxsize=None)
+def _graph_streams():
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'graph_streams.so')
+    if not os.path.exists(path):
+        raise ImportError('gcn_amd: %s is not built. Run `make -C gcn_amd/csrc` (or __graft_entry__.build()).' % path)
+    torch.ops.load_library(path)
+    return torch.ops.gcn_amd.graph_streams
+
+
 def _accumulators(*inputs):
     """The gradient accumulators of the leaves among the inputs, to be held over the call that uses them.  Refuses to record
     a differentiable call while an eager graph over the same leaves lives, those reached through other operations (a
     transposed weight) among them: such a graph keeps the accumulators, which belong to the stream it was built on, and a
-    backward pass recorded over them waits for that stream, which ends the capture and the process.  Eager calls
-    mark the nodes their inputs hang on; a mark dies with its node, that is, with the last eager graph that holds it."""
+    backward pass recorded over them waits for that stream, which ends the capture and the process.  Whoever built the eager
+    graph, its nodes' streams take no part in the recording.  Eager calls also mark the nodes their inputs hang on; a mark
+    dies with its node, that is, with the last eager graph that holds it."""
     held = []
     if not torch.is_grad_enabled():
         return held
     capturing, below = torch.cuda.is_current_stream_capturing(), []
+    if capturing:
+        tensors = [t for t in inputs if isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad]
+        streams = _graph_streams()(tensors) if tensors else ()
+        if not all(_records(*pair) for pair in zip(streams[::2], streams[1::2])):
+            _refuse_eager_graph()
     for t in inputs:
         if isinstance(t, torch.Tensor) and t.requires_grad:
             node = t.grad_fn
@@ -171,8 +205,7 @@ def _accumulators(*inputs):
         node = below.pop()
         if capturing:
             if node.metadata.get('gcn_amd_eager'):
-                raise RuntimeError('an eager autograd graph over an input of this recorded call is alive: drop its outputs '
-                                   'and losses before capturing')
+                _refuse_eager_graph()
             if node in seen:
                 continue
             seen.add(node)

@@ -262,3 +262,65 @@ def test_a_plan_of_two_streams():
             got.append(layers.quant_dot(a, x))
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def test_recording_over_eager_graphs_that_other_operations_built_is_refused():
+    """A leaf that plain torch operations hold, one held through a view, an eager operand: refused while the eager graph lives
+    (nothing is run backward there); afterwards the same calls record and replay."""
+    import torch
+    from gcn_amd import layers, metrics
+    gen = torch.Generator('cuda').manual_seed(3)
+    w = torch.randn((8, 8), device='cuda', generator=gen, requires_grad=True)
+    x = torch.randn((4, 8), device='cuda', generator=gen)
+    idx = torch.zeros((4, 1), dtype=torch.int32, device='cuda')
+    # warm-up, as a recording wants it
+    torch.autograd.grad(layers.dense(x, w, act='relu').sum() + layers.rms_norm(w).sum(), w)
+    for eager in (lambda: (w * w).sum(), lambda: w.t().exp(), lambda: layers.dot(x, w)):
+        alive = eager()
+        for call in (lambda: layers.dense(x, w, act='relu'), lambda: layers.dense(x, w.t()), lambda: layers.rms_norm(w),
+                     lambda: metrics.masked_distillation(w[:4], x[:, :1], idx, mask_mean=1.0)):
+            with pytest.raises(RuntimeError, match='eager autograd graph'):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    call()
+        del alive
+        torch.cuda.synchronize()
+    alive = w * 2
+    with pytest.raises(RuntimeError, match='eager autograd graph'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            layers.dense(x, alive)
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = torch.autograd.grad(layers.dense(x, w, act='relu').sum(), w)[0]
+    for _ in range(3):
+        graph.replay()
+        want = torch.autograd.grad(layers.dense(x, w, act='relu').sum(), w)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+
+
+def test_a_recorded_step_may_use_its_leaves_in_plain_operations_first():
+    """A decay term and a transposed weight recorded before the layer that uses the weight: graphs of the recording itself."""
+    import torch
+    from gcn_amd import layers
+    gen = torch.Generator('cuda').manual_seed(4)
+    w = torch.randn((8, 8), device='cuda', generator=gen, requires_grad=True)
+    x = torch.randn((4, 8), device='cuda', generator=gen)
+
+    def step():
+        decay = (w * w).sum()
+        out = layers.dense(layers.dense(x, w, act='silu'), w.t())
+        return torch.autograd.grad(out.sum() + decay, w)[0]
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step()
+    for _ in range(3):
+        with torch.no_grad():
+            w.normal_(generator=gen)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)

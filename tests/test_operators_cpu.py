@@ -256,3 +256,18 @@ def test_outputs_across_operands_are_refused():
         assert distill(**bad) == BAD, bad
     assert lib.gcn_quant_dense_f32(4, 6, Q, 16, S, Q + 60, 6, None) == BAD
     assert lib.gcn_quant_dense_f32(4, 6, Q, 16, S, S - 88, 6, None) == BAD
+
+
+def test_streams_of_host_graphs():
+    """The operator loads and walks a deep graph with shared nodes; host nodes belong to no stream, a leaf that nothing
+    holds has no node."""
+    import torch
+    from gcn_amd import layers
+    streams = layers._graph_streams()
+    w = torch.ones(3, requires_grad=True)
+    x = w
+    for _ in range(5000):
+        x = x + x
+    assert list(streams([w, x, torch.ones(2)])) == [] and list(streams([])) == []
+    del x
+    assert list(streams([w])) == []
