@@ -47,10 +47,15 @@ class _DistillationFn(torch.autograd.Function):
 def masked_distillation(preds, values, indices, mask=None, temperature=1.0, mask_mean=None):
     """(loss, agreement) of a model that learns from a teacher's top logits under the reference's mask: the mean over ALL
     rows of ``T^2 KL(teacher || student) * mask_i / mean(mask)``, and the same mean of whether the two arg maxima are the
-    same class.  ``values`` [n x k] are the teacher's logits of the classes ``indices`` (int32; outside the classes: no
-    entry), as ``sparse.distill_topk`` takes them.  Differentiable in ``preds``.  ``mask_mean``: mean(mask) as a number,
+    same class.  ``values`` [n x k] are the teacher's logits of the classes ``indices`` (int32, or int64 as ``torch.topk``
+    returns them; outside the classes: no entry), as ``sparse.distill_topk`` takes them.  ``mask`` [n]: bool, as the
+    reference's are, or whole numbers that weigh the rows.  Differentiable in ``preds``.  ``mask_mean``: mean(mask) as a number,
     if the caller has it -- taking it here waits for the device, which a recorded call cannot."""
     held = layers._accumulators(preds)        # noqa: F841 -- alive until the call below has its graph
+    if mask is not None and not (mask.is_floating_point() or mask.is_complex()):
+        mask = mask.to(torch.int32)
+    if indices.dtype == torch.int64:          # what int32 does not hold is no class either
+        indices = indices.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     if mask_mean is None:
         mask_mean = 1.0 if mask is None else float(mask.to(torch.float32).mean().item())
     return _DistillationFn.apply(preds, values, indices, mask, float(mask_mean), float(temperature))

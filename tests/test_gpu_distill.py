@@ -230,3 +230,27 @@ def test_empty_and_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_masks_and_indices_as_the_framework_and_topk_give_them():
+    """Bool masks and int64 indices through the loss, equal to the int32 ones bit for bit; an index past 32 bits is no
+    entry, a mask of fractions and indices of another kind are refused."""
+    import torch
+    from gcn_amd import metrics
+    logits, values, idx, mask = _case(300, 40, 5)
+    logits.requires_grad_(True)
+    idx[3, 1], idx[4, 2] = -1, 40
+    want = metrics.masked_distillation(logits, values, idx, mask, temperature=2.0)
+    grad = torch.autograd.grad(want[0], logits)[0]
+    far = idx.long()
+    far[3, 1], far[4, 2] = 2 ** 32 + 3, -2 ** 40 + 1
+    for m in (mask.bool(), mask.long(), mask.to(torch.uint8)):
+        got = metrics.masked_distillation(logits, values, far, m, temperature=2.0)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(torch.autograd.grad(got[0], logits)[0], grad)
+    for bad in (lambda: metrics.masked_distillation(logits, values, idx, mask.float()),
+                lambda: metrics.masked_distillation(logits, values, idx.float(), mask),
+                lambda: metrics.masked_distillation(logits, values, idx, mask.bool()[:299], mask_mean=1.0),
+                lambda: metrics.masked_distillation(logits, values, idx, torch.zeros_like(mask).bool())):
+        with pytest.raises(ValueError):
+            bad()
