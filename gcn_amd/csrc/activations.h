@@ -70,7 +70,7 @@ __device__ __forceinline__ void with_act(int act, F f) {
 // The epilogue of a dense layer: C = act(A . B + bias) + residual, the pre-activation A . B + bias kept in pre.
 struct EpiArgs {
     const float* bias;       // [n], may be null
-    const float* residual;   // [m x n], may be null; may be C itself
+    const float* residual;   // [m x n], may be null; may be C itself: the lane that stores an element has read it
     int64_t ldr;
     float* pre;              // [m x n], may be null
     int64_t ldp;

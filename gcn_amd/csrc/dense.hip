@@ -483,8 +483,8 @@ __global__ __launch_bounds__(kBlock, 3) void gemm_mfma_kernel(int64_t m, int64_t
             __syncthreads();
         }
     } else {
-        // edge tile in n (a narrow output).  With load_b_guarded in load_b_edge's place: 1M x 256 x 47 455 us against 400,
-        // 652,304 x 902 x 17 685 against 610
+        // edge tile in n (a narrow output): 2^20 x 256 x 47 360 us, 652,304 x 902 x 17 533; with load_b_guarded in
+        // load_b_edge's place 12 to 14 % more
         for (; t + 1 < n_edge; ++t) {
             load_a_fast((t + 1) * kBK);
             load_b_edge((t + 1) * kBK);
@@ -683,7 +683,8 @@ __host__ __device__ constexpr int ragged_stages(int64_t n, int64_t k, bool trans
 // RAGGED (EPI == kEpiLayer): any m, n and k and any alignment.  Rows of A past the end (and columns of B past n) repeat
 // the last one -- what they give is not stored --, and the last of k, loaded element by element with zeros past the
 // end, come after n_ktiles whole stages (ragged_stages): every address lies inside the operands, and the main loop has no test.
-// The guarded kernel ran 150,001 x 500 x 256 at 100 TFLOP/s, this one at 113, and its gradient
+// The guarded kernel ran 150,001 x 500 x 256 at 100 TFLOP/s, this one at 113 to 118 (105 in a training step, which stores
+// the pre-activation too), and its gradient
 // 150,001 x 256 x 500 (B [n x k]) at 114 instead of 97.  Same order of additions.  (With the last stage as a branch of
 // the loop and the first one peeled the kernel took 168 registers, three waves a SIMD instead of four: 109 TFLOP/s.)
 template <bool TRANS_B, int EPI, bool A_MASK = false, bool RAGGED = false>

@@ -10,7 +10,7 @@
 // four or eight classes each, so that a wave holds 64 / G rows and the reductions a row needs are shared by them; wider
 // ones to a wave or a workgroup, up to 32,768 classes; beyond that the row is read a second time for its gradient.
 // Measured, compulsory bytes over time (a large copy: 4.7 TB/s): 4 M x 47 classes, 5 listed: 390 us, 4.5 TB/s;
-// 4 M x 7, 3 listed: 90 us, 4.0; 1 M x 200, 20 listed: 389 us, 4.7; 8,192 x 32,768, 32 listed: 416 us, 5.2;
+// 4 M x 7, 3 listed: 90 us, 4.0; 1 M x 200, 20 listed: 354 to 389 us, 4.7 (546 where nearly every list names a class twice); 8,192 x 32,768, 32 listed: 416 us, 5.2;
 // read twice, 2,048 x 65,536: 292 us, 3.7 (held in registers, which then spill, 426 us); 8,192 x 32,768 read twice: 497 us.
 #include <algorithm>
 #include <hip/hip_fp16.h>

@@ -11,10 +11,11 @@
 // its result, and is written once.  A row of f columns belongs to G lanes (G a power of two; a wave holds 64 / G
 // rows) or, past 1024 columns, to a whole workgroup; lane l holds the columns 4 (l + G j) .. + 3, so that an
 // instruction of a group reads 16 G consecutive bytes.  Sums, the maximum and the weight's gradient are float32.
-// Measured, compulsory bytes over time (a large copy: 4.7 TB/s), rows of 1 GB: 8-bit output with residual 4.8 to 5.2 TB/s at
-// 16, 64, 256, 500, 1433, 2048 and 8192 columns (100: 4.0, whose 112 of 128 bytes a row are partial lines), float32 output
-// 4.9 to 5.3, gradients 4.3 to 5.0; past 16,384 columns 3.6 to 4.4 forward, and the gradient, which reads its rows twice there,
-// 2.5 to 3.2 (1.4 with the rows held in registers, which then spill).
+// Measured, compulsory bytes over time (a large copy: 4.7 TB/s), rows of 1 GB: 8-bit output with residual 4.9 to 5.4 TB/s at
+// 16, 64, 256, 500, 1433, 2048, 8192, 9000, 12,000 and 16,384 columns (100: 4.0, whose 112 of 128 bytes a row are partial
+// lines), float32 output 4.9 to 5.7, gradients 4.4 to 5.1 up to 8192 columns and 3.4 (9000) to 4.4 (16,384) up to 16,384, where
+// the kernel spills 11 registers; past that 3.6 to 5.2 forward, and the gradient, which reads its rows twice there,
+// 2.5 to 3.3 (1.4 with everything in registers).
 // A wave a row at 1433 columns (eight vectors a lane, two waves a SIMD) ran the gradient at 2.6 instead of 4.7.
 #include <algorithm>
 
@@ -246,9 +247,10 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_grad_kernel(NormGradArgs a, in
     }
 }
 
-// Rows past 16,384 columns, a workgroup a row: two of its operands and the weight's gradient do not fit the 128 registers of
-// a lane among 1024 (the kernel above spilled 338 of them).  The weight's gradient stays in LDS, every lane at its own
-// columns, and the row is read a second time, from the caches, for dx.
+// Rows past 16,384 columns, a workgroup a row: two of its operands, the weight and its gradient do not fit the 128 registers
+// of a lane among 1024 (the kernel above spilled 338 of them).  The weight's gradient stays in LDS, every lane at its own
+// columns, and the row is read a second time, from the caches, for dx.  (The two operands alone would be 64 registers a lane:
+// a form that keeps them has not been built.)
 __global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(NormGradArgs a, int tile) {
     constexpr int G = 1024, kDepth = 4;
     __shared__ float lds[2][16];

@@ -12,8 +12,10 @@
 // 8 of its 16 columns, then 4, 2, 1.  Long rows are cut at the chunks of the wide dense product and joined in chunk order.
 // Measured (R-MAT, 32 entries a row; rows gathered + compulsory bytes over time; random row gathers end at 7.5 TB/s):
 // 2^20 nodes x 256: 1.29 ms, 7.5 TB/s (float32 rows: 3.92 ms); x 512: 2.54 (8.34); x 128: 0.81 (1.93); x 16: 0.58 (0.56).
-// 2^24 nodes x 256: 28.5 ms (74.6), x 128: 18.9 (39.0), x 64: 18.1 (20.0), x 16: 16.7 (10.7): there the 64 MB of scales no
-// longer stay in the L2s and every entry pays a line for its scale, so rows of 64 columns and fewer are for small graphs.
+// 2^24 nodes x 256: 28.5 ms (74.6), x 128: 18.9 (39.0), x 64: 18.2 (20.1), x 32: 17.5 (11.1), x 16: 16.8 (10.7): there the
+// 64 MB of scales no longer stay in the L2s and every entry pays a line for its scale, so rows of 32 columns and fewer are for
+// graphs of up to about 2^20 nodes (2^22 x 32: 3.4 ms against 2.5, x 64: 3.8 against 4.5).
+// At six waves a SIMD the kernel spills 3 to 13 registers where rows of 33 to 128 or more than 256 columns are gathered.
 // Steps tried on 2^20 x 256 / 2^24 x 256: a row after the other, every row's loads drained before the next row's
 // 1.62 / 33.8 ms; the stream below with 4 steps in flight 1.38 / 28.8, with 8 (4 waves a SIMD) 1.55 / 30.3, with 2 and 6 waves
 // a SIMD 1.29 / 28.5; non-temporal row loads 1.95 / 32.3 (the hubs' rows leave the L2).
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(kBlock, 6) void spmm_quant_kernel(PlanView pv, cons
     }
 }
 
-// y <- the float32 values an 8-bit matrix stands for, four columns a thread
+// y <- the float32 values an 8-bit matrix stands for, four columns a thread: 2^20 x 256 494 us, 2.7 TB/s (single stores, a
+// division for the row)
 __global__ __launch_bounds__(kBlock) void quant_dense_kernel(int64_t n_rows, int f, const uint8_t* __restrict__ q, int64_t ldq,
                                                              const float* __restrict__ scales, float* __restrict__ y,
                                                              int64_t ldy) {

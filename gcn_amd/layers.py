@@ -357,7 +357,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 def quant_dot(support, x, weight=None, residual=None, eps=1e-6, fuse_relu=False):
     """``dot(support, rms_norm(x, ...), sparse=True)`` with the normalised rows in 8 bits (a scale a row): the product
     gathers a quarter of the bytes.  Returns ``out``, or ``(out, h)`` with a residual.  Differentiable in x, weight and
-    residual; the rounding to 8 bits passes the gradient on unchanged."""
+    residual; the rounding to 8 bits passes the gradient on unchanged, and the backward product gathers float32 rows.
+    Rows of 32 columns and fewer are slower in 8 bits from about 2^22 nodes on (2^24 nodes of 16 columns: 16.8 ms against
+    10.7 for the product): there every entry pays a line for its row's scale."""
     held = _accumulators(x, weight, residual)        # noqa: F841 -- alive until the call below has its graph
     return _QuantDotFn.apply(support, x, weight, residual, float(eps), bool(fuse_relu))
 
