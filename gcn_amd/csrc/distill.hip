@@ -584,7 +584,8 @@ int gcn_distill_topk_f32(int64_t n, int64_t c, const float* logits, int64_t ldx,
     if (value_type != GCN_F32 && value_type != GCN_F16 && value_type != GCN_BF16)
         return fail(GCN_ERR_BAD_ARG, "unknown type %d of the teacher's logits", value_type);
     if (!(mask_mean > 0.0f)) return fail(GCN_ERR_BAD_ARG, "mask_mean must be positive (an empty mask has no loss)");
-    if (!(temperature > 0.0f) || !(temperature < INFINITY)) return fail(GCN_ERR_BAD_ARG, "the temperature must be positive");
+    if (!(temperature > 0.0f) || !(temperature < INFINITY) || !(1.4426950408889634f / temperature < INFINITY))
+        return fail(GCN_ERR_BAD_ARG, "the temperature must be positive, and its inverse a float32 number");
     if (n == 0) return GCN_OK;
     if (!logits || !values || !indices) return fail(GCN_ERR_BAD_ARG, "null pointer");
     if (row_stats && ((uintptr_t)row_stats & 7)) return fail(GCN_ERR_BAD_ARG, "row_stats must be 8-byte aligned");

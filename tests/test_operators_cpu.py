@@ -271,3 +271,9 @@ def test_streams_of_host_graphs():
     assert list(streams([w, x, torch.ones(2)])) == [] and list(streams([])) == []
     del x
     assert list(streams([w])) == []
+
+
+def test_distillation_refuses_a_temperature_without_an_inverse():
+    """A logit of the maximum times an infinite 1 / T would be NaN."""
+    for temp in (1e-45, 1e-39, 4e-39):
+        assert _distill(x=P, v=P + (1 << 16), i=P + (2 << 16), mask=P + (3 << 16), stats=P + (4 << 16), d=P + (5 << 16), temp=temp) == BAD
